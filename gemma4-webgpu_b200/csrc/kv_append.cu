@@ -1,0 +1,312 @@
+// q4k_kv_append: keys and values of new tokens into the paged 8-bit cache
+// (kv_cache.cuh), keys -- and queries, when given -- rotated by their
+// positions on the way.  The reference keeps an f32 cache and runs one pass
+// each for the rotation and the two stores (shaders/rope.wgsl:1-22,
+// shaders/kv_cache_store.wgsl:1-18).
+//
+//   rotation of pair j < R/2 at position p, (c, s) = rope[p][j]:
+//     x'_j       = x_j c - x_{j+R/2} s
+//     x'_{j+R/2} = x_{j+R/2} c + x_j s        (elements past R unchanged)
+//   block scale 2^E over the block's 16 tokens (those already there keep
+//     theirs: E never falls while the block fills), code = e4m3(x' / 2^E),
+//     nearest even; a block whose scale changes has its other slots recoded.
+//
+// One CTA owns one block of one sequence and head: its new rows stay in
+// registers (16 values a thread) between the maximum and the codes, so k, v
+// are read once and the codes written once, and nothing is shared between
+// CTAs.  Only when the scale changes are the block's other codes read back.
+// What bounds it is the traffic: 2 reads + 1 write of 8 bits per value.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "kv_cache.cuh"
+
+namespace q4k {
+namespace {
+
+constexpr uint32_t kQHeadsPerCta = 4;  // query heads that share a thread's (cos, sin)
+
+struct AppendArgs {
+  KvCache c;
+  KvBatch b;
+  const void* k;
+  const void* v;
+  const void* q;
+  void* q_out;
+  uint64_t k_stride, v_stride, q_stride, qo_stride;
+  uint32_t q_heads;
+  const float* rope;  // [rope_len][R / 2][2]
+  uint32_t rope_len, rot;
+  uint32_t* status;
+};
+
+// The 8 + 8 elements of a row that a thread's item holds: item i of D / 16.
+// Rotated ones are 8 pairs (lo, lo + R/2); the others 16 in a row.
+__device__ __forceinline__ void item_at(uint32_t i, uint32_t rot, uint32_t* lo, uint32_t* hi) {
+  if (8 * i < rot / 2) {
+    *lo = 8 * i;
+    *hi = 8 * i + rot / 2;
+  } else {
+    *lo = 16 * i;
+    *hi = 16 * i + 8;
+  }
+}
+
+__device__ __forceinline__ void rotate8(float (&a)[8], float (&b)[8], const float4* cs) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float4 t = cs[j];  // two pairs' (cos, sin)
+    const float a0 = a[2 * j], b0 = b[2 * j], a1 = a[2 * j + 1], b1 = b[2 * j + 1];
+    a[2 * j] = __fsub_rn(__fmul_rn(a0, t.x), __fmul_rn(b0, t.y));
+    b[2 * j] = __fadd_rn(__fmul_rn(b0, t.x), __fmul_rn(a0, t.y));
+    a[2 * j + 1] = __fsub_rn(__fmul_rn(a1, t.z), __fmul_rn(b1, t.w));
+    b[2 * j + 1] = __fadd_rn(__fmul_rn(b1, t.z), __fmul_rn(a1, t.w));
+  }
+}
+
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], float inv) {
+  uint2 r;
+  r.x = e4m3x2(x[0] * inv, x[1] * inv) | (e4m3x2(x[2] * inv, x[3] * inv) << 16);
+  r.y = e4m3x2(x[4] * inv, x[5] * inv) | (e4m3x2(x[6] * inv, x[7] * inv) << 16);
+  return r;
+}
+
+// A code's value as e4m3 holds it without saturation: past 464, where
+// rounding leaves the largest finite code, it is NaN.
+__device__ __forceinline__ float unsaturated(float x) { return fabsf(x) > 464.0f ? __int_as_float(0x7fc00000) : x; }
+
+// The codes of 4 values under a scale 1 / ratio times the old one.
+__device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
+  const uint32_t a = e4m3_to_f16x2(w & 0xffffu), b = e4m3_to_f16x2(w >> 16);
+  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a));
+  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+  return e4m3x2(unsaturated(x.x * ratio), unsaturated(x.y * ratio)) |
+         (e4m3x2(unsaturated(y.x * ratio), unsaturated(y.y * ratio)) << 16);
+}
+
+// A value as the cache can hold it: +-inf the largest, NaN zero (both are
+// reported); so no code at a position of a sequence is ever NaN.
+__device__ __forceinline__ float finite(float x, bool* bad) {
+  if (fabsf(x) <= 3.402823466e38f) return x;
+  *bad = true;
+  return x != x ? 0.0f : copysignf(3.402823466e38f, x);
+}
+
+// grid.x: block slots (sequence b's start at q_start[b] / 16 + 2 b, which
+// leaves each sequence room for every block that its n tokens can touch, so
+// no prefix sum is needed); grid.y: key heads, value heads, groups of query
+// heads.  blockDim.x = head dim: one item (16 values) of one token a thread.
+template <typename T>
+__global__ void __launch_bounds__(512) append_kernel(const AppendArgs a) {
+  const uint32_t D = a.c.dim, H = a.c.heads, per = D / 16;
+  uint32_t b = 0;
+  for (uint32_t i0 = 0; i0 < a.b.seqs; i0 += blockDim.x) {
+    const uint32_t i = i0 + threadIdx.x;
+    b += __syncthreads_count(i < a.b.seqs && a.b.q_start[i] / 16 + 2 * i <= blockIdx.x);
+  }
+  if (b == 0) return;
+  --b;
+  const KvSeq s = kv_seq(a.b, a.c.page_shift, b);
+  if (s.bad) {
+    if (threadIdx.x == 0) atomicOr(a.status, kStatusKvMeta);
+    return;
+  }
+  if (s.n == 0) return;
+  // new tokens whose position would be negative (n > kv_len) are left out
+  const uint32_t skip = s.n > s.kv ? s.n - s.kv : 0;
+  const uint32_t p0 = s.kv - (s.n - skip);
+  const uint32_t bs = (p0 / 16 + blockIdx.x - (a.b.q_start[b] / 16 + 2 * b)) * 16;  // the block's first position
+  const bool range_bad = skip > 0 || (a.rot && s.kv > a.rope_len);
+  if (range_bad && threadIdx.x == 0) atomicOr(a.status, kStatusKvMeta);
+  if (bs >= s.kv) return;
+  const uint32_t pos = bs + threadIdx.x / per, item = threadIdx.x % per;
+  const bool mine = pos >= p0 && pos < s.kv && !(a.rot && pos >= a.rope_len);
+  const uint64_t row = s.t0 + skip + (pos - p0);
+  uint32_t role = blockIdx.y;
+  uint32_t lo, hi;
+  if (role >= 2 * H) {  // queries
+    if (!mine) return;
+    item_at(item, a.rot, &lo, &hi);
+    const bool turn = 8 * item < a.rot / 2;
+    float4 cs[4];
+    if (turn) {
+      const float4* t = reinterpret_cast<const float4*>(a.rope + ((uint64_t)pos * (a.rot / 2) + 8 * item) * 2);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) cs[j] = __ldg(t + j);
+    }
+    const uint32_t h0 = (role - 2 * H) * kQHeadsPerCta;
+    const T* src = static_cast<const T*>(a.q) + row * a.q_stride;
+    T* dst = static_cast<T*>(a.q_out) + row * a.qo_stride;
+#pragma unroll
+    for (uint32_t h = h0; h < h0 + kQHeadsPerCta; ++h) {
+      if (h >= a.q_heads) break;
+      float x[8], y[8];
+      load_elems(src + h * D + lo, x);
+      load_elems(src + h * D + hi, y);
+      if (turn) rotate8(x, y, cs);
+      store_elems(dst + h * D + lo, x);
+      store_elems(dst + h * D + hi, y);
+    }
+    return;
+  }
+  const bool is_v = role >= H;
+  const uint32_t h = is_v ? role - H : role;
+  const uint32_t rot = is_v ? 0 : a.rot;
+  item_at(item, rot, &lo, &hi);
+  float x[8] = {}, y[8] = {};
+  bool bad = false;
+  float mx = 0.0f;
+  if (mine) {
+    const T* src = static_cast<const T*>(is_v ? a.v : a.k) + row * (is_v ? a.v_stride : a.k_stride) + h * D;
+    load_elems(src + lo, x);
+    load_elems(src + hi, y);
+    if (8 * item < rot / 2) {
+      const float4* t = reinterpret_cast<const float4*>(a.rope + ((uint64_t)pos * (rot / 2) + 8 * item) * 2);
+      float4 cs[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) cs[j] = __ldg(t + j);
+      rotate8(x, y, cs);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = finite(x[j], &bad);
+      y[j] = finite(y[j], &bad);
+      // an infinite element saturates and does not raise the others' scale
+      if (fabsf(x[j]) < 3.4e38f) mx = fmaxf(mx, fabsf(x[j]));
+      if (fabsf(y[j]) < 3.4e38f) mx = fmaxf(mx, fabsf(y[j]));
+    }
+  }
+  if (bad) atomicOr(a.status, kStatusKvNonFinite);
+  // the block's largest magnitude (as bits: they order like the values)
+  __shared__ uint32_t s_max[16];
+  const uint32_t wm = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = wm;
+  const uint32_t page = a.b.table[(uint64_t)b * a.b.cols + (bs >> a.c.page_shift)];
+  uint64_t blk;
+  const bool ok = kv_block(a.c, page, h, bs, &blk);
+  float* const sp = (is_v ? a.c.vs : a.c.ks) + blk;
+  const bool fresh = p0 <= bs;  // the block's first token comes now
+  const float old = ok ? *sp : 0.0f;
+  __syncthreads();
+  if (!ok) {
+    if (threadIdx.x == 0) atomicOr(a.status, kStatusKvMeta);
+    return;
+  }
+  uint32_t m = s_max[0];
+  for (uint32_t i = 1; i < blockDim.x / 32; ++i) m = max(m, s_max[i]);
+  int e = kv_scale_exp(__uint_as_float(m));
+  const int e_old = exp_of(old);
+  if (!fresh) e = max(e, e_old);
+  uint8_t* const base = (is_v ? a.c.v : a.c.k) + blk * (16 * D) + (uint64_t)(pos - bs) * D;
+  if (mine) {
+    const float inv = exp2i(-e);
+    *reinterpret_cast<uint2*>(base + lo) = codes8(x, inv);
+    *reinterpret_cast<uint2*>(base + hi) = codes8(y, inv);
+  } else if (e != e_old) {
+    // a slot without a new token: an older token's, or one past the end whose
+    // stale content a fresh block's smaller scale may not hold (then NaN; no
+    // position has it yet)
+    const float ratio = exp2i(min(max(e_old - e, -126), 127));
+    uint2* u = reinterpret_cast<uint2*>(base + lo);
+    uint2* w = reinterpret_cast<uint2*>(base + hi);
+    *u = make_uint2(recode4(u->x, ratio), recode4(u->y, ratio));
+    *w = make_uint2(recode4(w->x, ratio), recode4(w->y, ratio));
+  }
+  if (threadIdx.x == 0 && e != e_old) *sp = exp2i(e);
+}
+
+}  // namespace
+
+int kv_views(q4k_ctx* ctx, const char* what, const q4k_kv_cache* cache, const q4k_kv_batch* batch, uint32_t dtype,
+             uint32_t q_heads, KvCache* c, KvBatch* b) {
+  if (!cache || !batch) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "%s: null cache or batch", what);
+  if (!cache->k || !cache->v || !cache->k_scale || !cache->v_scale || !batch->block_table || !batch->q_start ||
+      !batch->kv_len)
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (dtype > Q4K_BF16) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "%s: unknown dtype %u", what, dtype);
+  const uint32_t D = cache->head_dim, P = cache->page_size;
+  if (D != 64 && D != 128 && D != 256 && D != 512)
+    return ctx_fail(ctx, Q4K_ERR_UNSUPPORTED, "%s: head_dim=%u is not 64, 128, 256 or 512", what, D);
+  if (P < 16 || P > 1024 || (P & (P - 1)))
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "%s: page_size=%u is not a power of two in [16, 1024]", what, P);
+  if (cache->pages == 0 || cache->kv_heads == 0 || cache->kv_heads > 1024)
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "%s: pages=%u kv_heads=%u out of range", what, cache->pages,
+                    cache->kv_heads);
+  if (!aligned16(cache->k) || !aligned16(cache->v))
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "%s: cache codes must be 16-byte aligned", what);
+  if (q_heads % cache->kv_heads != 0 || q_heads > 64 * cache->kv_heads)
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "%s: q_heads=%u is not 1..64 times kv_heads=%u", what, q_heads,
+                    cache->kv_heads);
+  if (batch->table_cols == 0 || (uint64_t)batch->table_cols * P >= (1ull << 31))
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "%s: table_cols=%u out of range", what, batch->table_cols);
+  if (batch->seqs > 65536 || batch->tokens > (1u << 24))
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "%s: seqs=%u (at most 65536) tokens=%u (at most 2^24) out of range",
+                    what, batch->seqs, batch->tokens);
+  c->k = static_cast<uint8_t*>(cache->k);
+  c->v = static_cast<uint8_t*>(cache->v);
+  c->ks = cache->k_scale;
+  c->vs = cache->v_scale;
+  c->pages = cache->pages;
+  c->page_shift = (uint32_t)__builtin_ctz(P);
+  c->heads = cache->kv_heads;
+  c->dim = D;
+  b->table = batch->block_table;
+  b->q_start = batch->q_start;
+  b->kv_len = batch->kv_len;
+  b->seqs = batch->seqs;
+  b->tokens = batch->tokens;
+  b->cols = batch->table_cols;
+  return Q4K_OK;
+}
+
+}  // namespace q4k
+
+using namespace q4k;
+
+extern "C" int q4k_kv_append(q4k_ctx* ctx, const q4k_kv_cache* cache, const q4k_kv_batch* batch, uint32_t dtype,
+                             const void* k, uint64_t k_stride, const void* v, uint64_t v_stride, const float* rope,
+                             uint32_t rope_len, uint32_t rope_dim, const void* q, uint64_t q_stride, void* q_out,
+                             uint64_t q_out_stride, uint32_t q_heads, void* stream) {
+  if (!ctx) return Q4K_ERR_INVALID_ARG;
+  AppendArgs a{};
+  const int rc = kv_views(ctx, "q4k_kv_append", cache, batch, dtype, q ? q_heads : 0, &a.c, &a.b);
+  if (rc != Q4K_OK) return rc;
+  if (a.b.tokens == 0 || a.b.seqs == 0) {
+    ctx->err[0] = 0;
+    return Q4K_OK;
+  }
+  if (!k || !v || (q && (!q_out || q_heads == 0)))
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_kv_append: null pointer");
+  const uint32_t D = a.c.dim;
+  if (rope_dim % 16 != 0 || rope_dim > D || (rope_dim && (!rope || rope_len == 0)))
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG,
+                    "q4k_kv_append: rope_dim=%u must be a multiple of 16 up to head_dim=%u, with a table", rope_dim, D);
+  if (rope_dim && !aligned16(rope)) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_kv_append: rope must be 16-byte aligned");
+  const uint64_t kv_row = (uint64_t)a.c.heads * D, q_row = (uint64_t)q_heads * D;
+  if (!rows_ok(k, k_stride, kv_row, dtype) || !rows_ok(v, v_stride, kv_row, dtype) ||
+      (q && (!rows_ok(q, q_stride, q_row, dtype) || !rows_ok(q_out, q_out_stride, q_row, dtype))))
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG,
+                    "q4k_kv_append: rows must be 16-byte aligned and at least heads * head_dim elements apart");
+  a.k = k;
+  a.v = v;
+  a.q = q;
+  a.q_out = q_out;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.q_stride = q_stride;
+  a.qo_stride = q_out_stride;
+  a.q_heads = q ? q_heads : 0;
+  a.rope = rope;
+  a.rope_len = rope_len;
+  a.rot = rope_dim;
+  a.status = ctx->select.status;
+  const dim3 grid(a.b.tokens / 16 + 2 * a.b.seqs + 1, 2 * a.c.heads + (a.q_heads + kQHeadsPerCta - 1) / kQHeadsPerCta);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == Q4K_F32)
+    append_kernel<float><<<grid, D, 0, st>>>(a);
+  else if (dtype == Q4K_F16)
+    append_kernel<__half><<<grid, D, 0, st>>>(a);
+  else
+    append_kernel<__nv_bfloat16><<<grid, D, 0, st>>>(a);
+  return ctx_cuda(ctx, cudaGetLastError(), "q4k_kv_append launch");
+}

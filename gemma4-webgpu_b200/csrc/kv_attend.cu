@@ -1,0 +1,675 @@
+// q4k_paged_attention for few rows per sequence (a decode step): attention
+// over the paged 8-bit cache (kv_cache.cuh).  The reference runs three passes
+// over an f32 cache (shaders/attn_score.wgsl:14-39, softmax.wgsl,
+// attn_output.wgsl:10-22); this is one pass with running softmax statistics.
+//
+// Mathematics.  With s_j the base-2 logits of a row and 2^e_j the value scale
+// of key j's block, let t_j = s_j + e_j and m the running maximum of t.  Then
+//   p_j = 2^(t_j - m),   O = sum_j p_j code_j,   l = sum_j p_j 2^(-e_j),
+// and the row's output is O / l: the value scales enter as additions to
+// exponents, so the value codes are used as they are, and m follows the terms
+// that matter to O.  Key scales and the row's own scale multiply the score.
+//
+// Work.  A unit is one sequence, key head and group of 8 * NT rows (rows of a
+// sequence: token-major, the query heads that share the key head within).
+// All units' 16-key blocks, laid end to end, are cut into equal ranges, one
+// per CTA, so a few long sequences and many short ones both fill the GPU.
+// In a CTA each warp takes every kWarps-th block of the range on its own (its
+// own copy ring, statistics and accumulators, no barrier in the loop); the
+// warps' results are added in shared memory, and a unit that was cut is
+// merged by the CTA that finishes last, in the order of the parts, so results
+// do not depend on timing.
+//
+// Products run on mma.sync (keys or value dims as M = 16, rows as N = 8): the
+// kernel is bound by reading the cache, and with 8 rows an M = 128 tcgen05
+// tile would be 1/16 full.  Codes are converted to f16, which is exact.  A
+// row enters as f16 after a power-of-two scale, which holds f16 and bf16 rows
+// exactly; f32 rows enter as f16 hi + lo (22 bits), and so do their
+// probabilities, so that f32 results hold f32 accuracy.  For f16 and bf16
+// rows the probabilities are rounded once to f16's 11 bits: less than the
+// output's own rounding.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "kv_attend.cuh"
+#include "kv_cache.cuh"
+#include "q4k_ptx.cuh"
+
+namespace q4k {
+namespace {
+
+constexpr float kPShift = 14.0f;  // probabilities are stored times 2^14: f16 then holds them down to 2^-28 in full
+constexpr uint32_t kMergeGroup = 16;
+
+template <int D>
+struct AttendCfg {
+  static constexpr int kWarps = D == 512 ? 4 : 8;
+  static constexpr int kStages = D >= 256 ? 3 : 4;
+  static constexpr int kRow = D + 16;                    // bytes of a staged row: the pad spreads rows over the banks
+  static constexpr int kStage = 2 * 16 * kRow + 16;      // 16 keys, 16 values, their scales
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kVec = D >= 128 ? 16 : 8;         // bytes of a value row a thread takes at a time
+  static constexpr int kPasses = D / (8 * kVec);         // value passes of 8 threads x kVec bytes
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
+
+// 2^(m - top), 0 for an empty part.
+__device__ __forceinline__ float part_weight(float m, float top) { return m == neg_inf() ? 0.0f : ex2(m - top); }
+
+struct Seg {  // a sequence's share of the work
+  KvSeq s;
+  uint32_t first, blocks, groups;  // first 16-key block, blocks, row groups
+};
+
+template <int R>
+__device__ __forceinline__ Seg seq_work(const AttendArgs& a, uint32_t b) {
+  Seg w;
+  w.s = kv_seq(a.b, a.c.page_shift, b);
+  const uint32_t rows = w.s.n * a.group;
+  w.groups = (rows + R - 1) / R;
+  if (a.max_rows && rows > a.max_rows) w.groups = 0;  // a prompt: the tile kernel's
+  const int low = a.window ? (int)w.s.kv - (int)w.s.n - (int)a.window + 1 : 0;
+  w.first = low > 0 ? (uint32_t)low / 16 : 0;
+  w.blocks = (w.s.kv + 15) / 16 - min(w.first, (w.s.kv + 15) / 16);
+  return w;
+}
+
+template <int D, int NT, typename T>
+__global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, 1) attend_kernel(const AttendArgs a) {
+  using C = AttendCfg<D>;
+  constexpr bool kHiLo = Elem<T>::kExact;
+  constexpr int R = 8 * NT;  // rows of a unit
+  constexpr int kThreads = C::kWarps * 32;
+  constexpr int kQStep = 32 * (kHiLo ? 16 : 8);  // bytes of one k-step's row operand
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint8_t* const ring = smem;
+  uint8_t* const qf = smem + C::kRing;  // [D / 16][NT][32 lanes] row operand in fragment order
+  __shared__ float s_rs[R], s_m[C::kWarps][R], s_l[C::kWarps][R], s_f[2 * kMergeGroup][R], s_tot[R];
+  __shared__ unsigned long long s_scan[C::kWarps + 1];
+  __shared__ unsigned long long s_off;
+  __shared__ uint32_t s_seq, s_last;
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
+  const uint32_t H = a.c.heads, G = a.group;
+
+  // rows that see nothing, and sequences that cannot be served
+  for (uint32_t b = blockIdx.x; b < a.b.seqs; b += gridDim.x) {
+    const Seg w = seq_work<R>(a, b);
+    if (w.s.bad && tid == 0) atomicOr(a.status, kStatusKvMeta);
+    if (w.groups && w.blocks == 0) {
+      const uint32_t per = a.c.heads * G * D;
+      for (uint64_t i = tid; i < (uint64_t)w.s.n * per; i += kThreads)
+        static_cast<T*>(a.out)[(w.s.t0 + i / per) * a.out_stride + i % per] = Elem<T>::from(0.0f);
+    }
+  }
+
+  // this CTA's range of the blocks of all units: each thread sums a run of
+  // sequences, a scan over the threads finds the one the range starts in
+  const uint32_t per_thread = (a.b.seqs + kThreads - 1) / kThreads;
+  const uint32_t b_lo = min(tid * per_thread, a.b.seqs), b_hi = min(b_lo + per_thread, a.b.seqs);
+  unsigned long long mine = 0;
+  for (uint32_t b = b_lo; b < b_hi; ++b) {
+    const Seg w = seq_work<R>(a, b);
+    mine += (unsigned long long)w.blocks * w.groups * H;
+  }
+  unsigned long long scan = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long up = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= (uint32_t)o) scan += up;
+  }
+  if (lane == 31) s_scan[warp + 1] = scan;
+  if (tid == 0) s_scan[0] = 0;
+  __syncthreads();
+  unsigned long long total = 0, before = scan - mine;
+#pragma unroll
+  for (int i = 0; i < C::kWarps; ++i) {
+    total += s_scan[i + 1];
+    if (i < (int)warp) before += s_scan[i + 1];
+  }
+  if (total == 0) return;
+  // at least kWarps blocks a CTA: fewer leave warps idle and make more parts to merge
+  unsigned long long n_cta = (total + C::kWarps - 1) / C::kWarps;
+  n_cta = n_cta < gridDim.x ? n_cta : gridDim.x;
+  if (blockIdx.x >= n_cta) return;
+  unsigned long long cur = total * blockIdx.x / n_cta;
+  const unsigned long long end = total * (blockIdx.x + 1) / n_cta;
+  if (cur >= before && cur < before + mine) {
+    unsigned long long o = before;
+    for (uint32_t b = b_lo; b < b_hi; ++b) {
+      const Seg w = seq_work<R>(a, b);
+      const unsigned long long c = (unsigned long long)w.blocks * w.groups * H;
+      if (cur < o + c) {
+        s_seq = b;
+        s_off = o;
+        break;
+      }
+      o += c;
+    }
+  }
+  __syncthreads();
+  uint32_t b = s_seq;
+  unsigned long long seq0 = s_off;  // global index of sequence b's first block
+
+  const uint32_t row_k = (g >> 1) + 4 * (g & 1);  // the key (of 8) that fragment row g holds: conflict-free with kRow
+  const uint32_t ring_u = smem_u32(ring) + warp * C::kStages * C::kStage;
+
+  while (cur < end) {
+    const Seg w = seq_work<R>(a, b);
+    const unsigned long long cnt = (unsigned long long)w.blocks * w.groups * H;
+    if (cur >= seq0 + cnt) {
+      seq0 += cnt;
+      ++b;
+      continue;
+    }
+    const uint32_t unit = (uint32_t)((cur - seq0) / w.blocks), u_off = (uint32_t)((cur - seq0) % w.blocks);
+    const uint32_t h = unit / w.groups, rg = unit % w.groups;
+    const uint32_t n_blk = (uint32_t)min((unsigned long long)(w.blocks - u_off), end - cur);
+    const uint32_t blk0 = w.first + u_off;
+    const uint32_t row0 = rg * R, n_rows = min((uint32_t)R, w.s.n * G - row0);
+    const int pos0 = (int)w.s.kv - (int)w.s.n;
+
+    // ---- the copy ring: warp w takes blocks blk0 + w, + kWarps, ... -----------
+    const uint32_t n_mine = n_blk > warp ? (n_blk - warp + C::kWarps - 1) / C::kWarps : 0;
+    const uint32_t* const table = a.b.table + (uint64_t)b * a.b.cols;
+    auto page_of = [&](uint32_t i) {
+      return i < n_mine ? table[((blk0 + warp + i * C::kWarps) * 16) >> a.c.page_shift] : 0u;
+    };
+    auto issue = [&](uint32_t i, uint32_t page) {
+      if (i < n_mine) {
+        const uint32_t pos = (blk0 + warp + i * C::kWarps) * 16;
+        uint64_t blk;
+        bool ok = kv_block(a.c, page, h, pos, &blk);
+        if (!ok) {  // out of range: read nothing (zeros), report
+          if (lane == 0) atomicOr(a.status, kStatusKvMeta);
+          blk = 0;
+        }
+        const uint32_t st = ring_u + (i % C::kStages) * C::kStage;
+        const uint8_t* ks = a.c.k + blk * (16 * D);
+        const uint8_t* vs = a.c.v + blk * (16 * D);
+        // slots past the sequence's end are read as zeros, whatever they hold
+        const uint32_t rows = ok ? min(16u, w.s.kv - pos) : 0u;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          const uint32_t c = lane + 32 * j, r = c / (D / 16), x = c % (D / 16);
+          cp_async16(st + r * C::kRow + 16 * x, ks + 16 * c, r < rows);
+          cp_async16(st + 16 * C::kRow + r * C::kRow + 16 * x, vs + 16 * c, r < rows);
+        }
+        if (lane < 2) cp_async4(st + 32 * C::kRow + 4 * lane, (lane ? a.c.vs : a.c.ks) + blk);
+      }
+      cp_commit();
+    };
+    uint32_t page_next = page_of(0);
+#pragma unroll
+    for (int i = 0; i < C::kStages - 1; ++i) {
+      const uint32_t p = page_next;
+      page_next = page_of(i + 1);
+      issue(i, p);
+    }
+
+    // ---- the rows' operand: f16 (hi, lo) fragments under a power of two per row
+    for (uint32_t r = warp; r < (uint32_t)R; r += C::kWarps) {
+      float x[D / 32 < 4 ? 1 : D / 128][4];
+      float mx = 0.0f;
+      const uint32_t rr = row0 + r;
+      const T* src = static_cast<const T*>(a.q) + (uint64_t)(w.s.t0 + rr / G) * a.q_stride + (h * G + rr % G) * D;
+      constexpr int kChunks = D >= 128 ? D / 128 : 1;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        if (r < n_rows && lane * 4 < (uint32_t)D) {
+          load_elems(src + 128 * i + 4 * lane, x[i]);
+        } else {
+          x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float v = fabsf(x[i][j]);
+          if (v <= 3.402823466e38f) mx = fmaxf(mx, v);
+        }
+      }
+      const uint32_t mb = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
+      int e = 13 - ((int)(mb >> 23) - 127);  // the largest element in [2^13, 2^14)
+      e = mb == 0 ? 0 : min(max(e, -110), 110);
+      const float up = exp2i(e);
+      if (lane == 0) s_rs[r] = a.scale_log2 * exp2i(-e);
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const uint32_t d = 128 * i + 4 * lane;
+        if (d >= (uint32_t)D) break;
+        float v[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[j] = x[i][j] * up;
+          lo[j] = v[j] - __half2float(__float2half_rn(v[j]));
+        }
+        // dims d..d+3 are one thread's four of k-step (d / 64, (d % 16) / 4)
+        const uint32_t step = (d / 64) * 4 + (d % 16) / 4, ln = (r % 8) * 4 + (d % 64) / 16;
+        uint8_t* dst = qf + (step * NT + r / 8) * kQStep + ln * (kHiLo ? 16 : 8);
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f16(v[0], v[1]), pack_f16(v[2], v[3]));
+        if constexpr (kHiLo)
+          *reinterpret_cast<uint2*>(dst + 8) = make_uint2(pack_f16(lo[0], lo[1]), pack_f16(lo[2], lo[3]));
+      }
+    }
+    __syncthreads();
+
+    float rs[NT][2];
+    int pos_q[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t r = nt * 8 + 2 * t + x;
+        rs[nt][x] = s_rs[r];
+        pos_q[nt][x] = r < n_rows ? pos0 + (int)((row0 + r) / G) : -1;
+      }
+    const int pos_min = pos0 + (int)(row0 / G), pos_max = pos0 + (int)((row0 + n_rows - 1) / G);
+
+    float m[NT][2], l[NT][2], o[C::kPasses * (C::kVec / 4)][2][NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = neg_inf(), l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < C::kPasses * (C::kVec / 4); ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) o[i][j][nt][0] = o[i][j][nt][1] = o[i][j][nt][2] = o[i][j][nt][3] = 0.0f;
+
+    for (uint32_t i = 0; i < n_mine; ++i) {
+      cp_wait<C::kStages - 2>();
+      __syncwarp();
+      {
+        const uint32_t p = page_next;
+        page_next = page_of(i + C::kStages);
+        issue(i + C::kStages - 1, p);
+      }
+      const uint8_t* st = ring + warp * C::kStages * C::kStage + (i % C::kStages) * C::kStage;
+      const float2 sc = *reinterpret_cast<const float2*>(st + 32 * C::kRow);
+      const int pos = (int)((blk0 + warp + i * C::kWarps) * 16);
+
+      // scores: keys x rows, four chains
+      float s[2][NT][4];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[c][nt][0] = s[c][nt][1] = s[c][nt][2] = s[c][nt][3] = 0.0f;
+      const uint8_t* kp = st + row_k * C::kRow + 16 * t;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        const uint4 ka = lds128(kp + 64 * c), kb = lds128(kp + 8 * C::kRow + 64 * c);
+        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t a0 = e4m3_to_f16x2(wa[j] & 0xffffu), a2 = e4m3_to_f16x2(wa[j] >> 16);
+          const uint32_t a1 = e4m3_to_f16x2(wb[j] & 0xffffu), a3 = e4m3_to_f16x2(wb[j] >> 16);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint8_t* q = qf + ((c * 4 + j) * NT + nt) * kQStep + lane * (kHiLo ? 16 : 8);
+            if constexpr (kHiLo) {
+              const uint4 v = lds128(q);
+              mma16816(s[0][nt], a0, a1, a2, a3, v.x, v.y);
+              mma16816(s[1][nt], a0, a1, a2, a3, v.z, v.w);
+            } else {
+              const uint2 v = *reinterpret_cast<const uint2*>(q);
+              mma16816(s[j & 1][nt], a0, a1, a2, a3, v.x, v.y);
+            }
+          }
+        }
+      }
+
+      // running statistics; the probabilities as the second product's operand
+      const float ev = (float)exp_of(sc.y), inv_v = exp2i(-exp_of(sc.y));
+      const bool edge = pos + 15 > pos_min || (a.window && pos <= pos_max - (int)a.window);
+      uint32_t p_hi[NT][2], p_lo[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float tv[2][2], corr[2];  // [key half][row]
+        bool moved = false;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float cs = sc.x * rs[nt][x];
+          tv[0][x] = fmaf(s[0][nt][x] + s[1][nt][x], cs, ev);
+          tv[1][x] = fmaf(s[0][nt][2 + x] + s[1][nt][2 + x], cs, ev);
+          if (edge) {
+            const int j0 = pos + (int)row_k, last = pos_q[nt][x];
+            const int low = a.window ? last - (int)a.window : -1;
+            if (j0 > last || j0 <= low) tv[0][x] = neg_inf();
+            if (j0 + 8 > last || j0 + 8 <= low) tv[1][x] = neg_inf();
+          }
+          float mx = fmaxf(tv[0][x], tv[1][x]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float mn = fmaxf(m[nt][x], mx);
+          corr[x] = m[nt][x] == mn ? 1.0f : part_weight(m[nt][x], mn);
+          moved |= m[nt][x] != mn;
+          m[nt][x] = mn;
+          const float ref = mn == neg_inf() ? 0.0f : mn - kPShift;
+          tv[0][x] = ex2(tv[0][x] - ref);
+          tv[1][x] = ex2(tv[1][x] - ref);
+          l[nt][x] = fmaf(tv[0][x] + tv[1][x], inv_v, l[nt][x] * corr[x]);
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int k = 0; k < C::kPasses * (C::kVec / 4); ++k)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              o[k][j][nt][0] *= corr[0];
+              o[k][j][nt][2] *= corr[0];
+              o[k][j][nt][1] *= corr[1];
+              o[k][j][nt][3] *= corr[1];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t hi = pack_f16(tv[k][0], tv[k][1]);
+          p_hi[nt][k] = transpose8x8(hi);
+          if constexpr (kHiLo) {
+            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+            p_lo[nt][k] = transpose8x8(pack_f16(tv[k][0] - back.x, tv[k][1] - back.y));
+          }
+        }
+      }
+
+      // values: dims x rows.  Thread (g, t) holds the codes of keys t, t + 4,
+      // t + 8, t + 12 (the transposed fragments' order) for its dims.
+      const uint8_t* vp = st + (16 + t) * C::kRow + (C::kVec == 16 ? 16 * ((g >> 1) + 4 * (g & 1)) : 8 * g);
+#pragma unroll
+      for (int ps = 0; ps < C::kPasses; ++ps) {
+        uint32_t wv[4][C::kVec / 4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (C::kVec == 16) {
+            const uint4 v = lds128(vp + 4 * k * C::kRow + 128 * ps);
+            wv[k][0] = v.x, wv[k][1] = v.y, wv[k][2] = v.z, wv[k][3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(vp + 4 * k * C::kRow);
+            wv[k][0] = v.x, wv[k][1] = v.y;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < C::kVec / 4; ++j) {
+          const uint32_t lo01 = __byte_perm(wv[0][j], wv[1][j], 0x5140), hi01 = __byte_perm(wv[0][j], wv[1][j], 0x7362);
+          const uint32_t lo23 = __byte_perm(wv[2][j], wv[3][j], 0x5140), hi23 = __byte_perm(wv[2][j], wv[3][j], 0x7362);
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            const uint32_t x = d ? hi01 : lo01, y = d ? hi23 : lo23;
+            const uint32_t a0 = e4m3_to_f16x2(x & 0xffffu), a1 = e4m3_to_f16x2(x >> 16);
+            const uint32_t a2 = e4m3_to_f16x2(y & 0xffffu), a3 = e4m3_to_f16x2(y >> 16);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float(&acc)[4] = o[ps * (C::kVec / 4) + j][d][nt];
+              mma16816(acc, a0, a1, a2, a3, p_hi[nt][0], p_hi[nt][1]);
+              if constexpr (kHiLo) mma16816(acc, a0, a1, a2, a3, p_lo[nt][0], p_lo[nt][1]);
+            }
+          }
+        }
+      }
+    }
+    cp_wait<0>();
+    __syncthreads();  // every warp is done with its ring: it now holds the warps' results
+
+    // ---- add the warps' parts -------------------------------------------------
+    float* const so = reinterpret_cast<float*>(ring);  // [kWarps][R][D]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float v = l[nt][x];
+        v += __shfl_xor_sync(0xffffffffu, v, 4);
+        v += __shfl_xor_sync(0xffffffffu, v, 8);
+        v += __shfl_xor_sync(0xffffffffu, v, 16);
+        const uint32_t r = nt * 8 + 2 * t + x;
+        if (g == 0) {
+          s_m[warp][r] = m[nt][x];
+          s_l[warp][r] = v;
+        }
+#pragma unroll
+        for (int k = 0; k < C::kPasses * (C::kVec / 4); ++k) {
+          const uint32_t d = C::kVec == 16 ? 128 * (k / 4) + 16 * ((g >> 1) + 4 * (g & 1)) + 4 * (k % 4) : 8 * g + 4 * k;
+          *reinterpret_cast<float4*>(so + ((uint32_t)warp * R + r) * D + d) =
+              make_float4(o[k][0][nt][x], o[k][0][nt][2 + x], o[k][1][nt][x], o[k][1][nt][2 + x]);
+        }
+      }
+    __syncthreads();
+    if (tid < (uint32_t)R) {
+      float top = neg_inf(), sum = 0.0f;
+      for (int i = 0; i < C::kWarps; ++i) top = fmaxf(top, s_m[i][tid]);
+      for (int i = 0; i < C::kWarps; ++i) {
+        const float f = part_weight(s_m[i][tid], top);
+        s_f[i][tid] = f;
+        sum += s_l[i][tid] * f;
+      }
+      s_m[0][tid] = top;  // only this thread reads row tid's
+      s_tot[tid] = sum;
+    }
+    __syncthreads();
+
+    // a unit that lies within this CTA is written; a part of one goes to the workspace
+    const unsigned long long u0 = seq0 + (unsigned long long)unit * w.blocks, u1 = u0 + w.blocks;
+    const uint32_t c0 = (uint32_t)(((u0 + 1) * n_cta - 1) / total), c1 = (uint32_t)((u1 * n_cta - 1) / total);
+    const bool whole = c0 == c1;
+    constexpr uint32_t kSlot = R * (D + 2);
+    auto slot = [&](uint32_t i) {  // part i of this unit: CTA c0 keeps its last part apart from its first
+      return a.work + (size_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * kSlot;
+    };
+    auto put = [&](uint32_t r, uint32_t d, float4 v) {
+      const uint32_t rr = row0 + r;
+      const float x[4] = {v.x, v.y, v.z, v.w};
+      store_elems(static_cast<T*>(a.out) + (uint64_t)(w.s.t0 + rr / G) * a.out_stride + (h * G + rr % G) * D + d, x);
+    };
+    float* const my_slot = whole ? nullptr : slot(blockIdx.x - c0);
+    for (uint32_t i = tid; i < n_rows * (D / 4); i += kThreads) {
+      const uint32_t r = i / (D / 4), d = i % (D / 4) * 4;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int k = 0; k < C::kWarps; ++k) {
+        const float f = s_f[k][r];
+        const float4 y = *reinterpret_cast<const float4*>(so + ((uint32_t)k * R + r) * D + d);
+        v.x += y.x * f, v.y += y.y * f, v.z += y.z * f, v.w += y.w * f;
+      }
+      if (whole) {
+        const float tot = s_tot[r], inv = tot != 0.0f ? 1.0f / tot : 0.0f;  // nothing seen: zero; NaN stays
+        put(r, d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+      } else {
+        *reinterpret_cast<float4*>(my_slot + r * D + d) = v;
+      }
+    }
+    if (!whole) {
+      if (tid < n_rows) {
+        my_slot[R * D + 2 * tid] = s_m[0][tid];
+        my_slot[R * D + 2 * tid + 1] = s_tot[tid];
+      }
+      // merge in groups of kMergeGroup parts, then the groups: the last CTA to
+      // arrive at each reads the parts in their order
+      const uint32_t parts = c1 - c0 + 1, grp = (blockIdx.x - c0) / kMergeGroup;
+      uint32_t stride = 1, n = min(kMergeGroup, parts - grp * kMergeGroup), p0 = grp * kMergeGroup;
+      uint32_t* counter = a.counters + c0 + p0;
+      for (;;) {
+        __syncthreads();
+        if (tid == 0) {
+          __threadfence();
+          s_last = atomicAdd(counter, 1u) == n - 1;
+          if (s_last) *counter = 0;  // every part has arrived: ready for the next call
+        }
+        __syncthreads();
+        if (!s_last) break;
+        __threadfence();
+        for (uint32_t r = tid; r < n_rows; r += kThreads) {
+          float top = neg_inf(), sum = 0.0f;
+          for (uint32_t i = 0; i < n; ++i) top = fmaxf(top, __ldcg(slot(p0 + i * stride) + R * D + 2 * r));
+          for (uint32_t i = 0; i < n; ++i) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(slot(p0 + i * stride) + R * D + 2 * r));
+            const float f = part_weight(ml.x, top);
+            s_f[i][r] = f;
+            sum += ml.y * f;
+          }
+          s_m[0][r] = top;
+          s_tot[r] = sum;
+        }
+        __syncthreads();
+        const bool done = p0 == 0 && (stride > 1 || parts <= kMergeGroup);
+        for (uint32_t i = tid; i < n_rows * (D / 4); i += kThreads) {
+          const uint32_t r = i / (D / 4), d = i % (D / 4) * 4;
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+          for (uint32_t k = 0; k < n; ++k) {
+            const float f = s_f[k][r];
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(slot(p0 + k * stride) + r * D + d));
+            v.x += y.x * f, v.y += y.y * f, v.z += y.z * f, v.w += y.w * f;
+          }
+          if (done) {
+            const float tot = s_tot[r], inv = tot != 0.0f ? 1.0f / tot : 0.0f;
+            put(r, d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+          } else {
+            *reinterpret_cast<float4*>(slot(p0) + r * D + d) = v;  // each element read by this thread alone before
+          }
+        }
+        if (done) break;
+        if (tid < n_rows) {
+          slot(p0)[R * D + 2 * tid] = s_m[0][tid];
+          slot(p0)[R * D + 2 * tid + 1] = s_tot[tid];
+        }
+        n = (parts + kMergeGroup - 1) / kMergeGroup;
+        stride = kMergeGroup;
+        p0 = 0;
+        counter = a.counters + kAttendMaxCtas + c0;
+      }
+    }
+    cur += n_blk;
+    __syncthreads();  // shared memory is reused by the next segment
+  }
+}
+
+template <int D, int NT, typename T>
+cudaError_t launch(const AttendArgs& a, uint32_t grid, int device, cudaStream_t s) {
+  using C = AttendCfg<D>;
+  constexpr int kSmem = C::kRing + (D / 16) * NT * 32 * (Elem<T>::kExact ? 16 : 8);
+  static_assert(C::kWarps * 8 * NT * D * 4 <= C::kRing, "the warps' results fit the ring");
+  static std::atomic<uint8_t> attr_set[kAttrDevices];
+  const cudaError_t e = smem_attr_once(attr_set, device, attend_kernel<D, NT, T>, kSmem);
+  if (e != cudaSuccess) return e;
+  attend_kernel<D, NT, T><<<grid, C::kWarps * 32, kSmem, s>>>(a);
+  return cudaGetLastError();
+}
+
+// Two row groups a unit when sequences have more than 8 rows: the codes are
+// then converted once for 16 rows.  At head dim 512 one group's accumulators
+// already take half the registers.
+template <int D, typename T>
+cudaError_t launch_rows(const AttendArgs& a, uint32_t rows, uint32_t grid, int device, cudaStream_t s) {
+  if constexpr (D < 512) {
+    if (rows > 8) return launch<D, 2, T>(a, grid, device, s);
+  }
+  return launch<D, 1, T>(a, grid, device, s);
+}
+
+template <typename T>
+cudaError_t launch_dim(const AttendArgs& a, uint32_t rows, uint32_t grid, int device, cudaStream_t s) {
+  switch (a.c.dim) {
+    case 64: return launch_rows<64, T>(a, rows, grid, device, s);
+    case 128: return launch_rows<128, T>(a, rows, grid, device, s);
+    case 256: return launch_rows<256, T>(a, rows, grid, device, s);
+    default: return launch_rows<512, T>(a, rows, grid, device, s);
+  }
+}
+
+}  // namespace
+}  // namespace q4k
+
+using namespace q4k;
+
+extern "C" int q4k_paged_attention(q4k_ctx* ctx, const q4k_kv_cache* cache, const q4k_kv_batch* batch, uint32_t dtype,
+                                   const void* q, uint64_t q_stride, void* out, uint64_t out_stride, uint32_t q_heads,
+                                   uint32_t max_q, float scale, uint32_t window, void* stream) {
+  if (!ctx) return Q4K_ERR_INVALID_ARG;
+  AttendArgs a{};
+  const int rc = kv_views(ctx, "q4k_paged_attention", cache, batch, dtype, q_heads, &a.c, &a.b);
+  if (rc != Q4K_OK) return rc;
+  if (a.b.tokens == 0 || a.b.seqs == 0) {
+    ctx->err[0] = 0;
+    return Q4K_OK;
+  }
+  if (!q || !out) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: null pointer");
+  if (q_heads == 0) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: q_heads must be >= 1");
+  if (!(scale == scale) || fabsf(scale) > 3.402823466e38f)
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: scale must be finite");
+  if (window >= (1u << 31)) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: window=%u out of range", window);
+  const uint64_t row = (uint64_t)q_heads * a.c.dim;
+  if (!rows_ok(q, q_stride, row, dtype) || !rows_ok(out, out_stride, row, dtype))
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG,
+                    "q4k_paged_attention: rows must be 16-byte aligned and at least q_heads * head_dim elements apart");
+  a.q = q;
+  a.out = out;
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.group = q_heads / a.c.heads;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.window = window;
+  a.work = reinterpret_cast<float*>(ctx->xfrag);
+  a.counters = ctx->split_counters;
+  a.status = ctx->select.status;
+  // prompts go to the tile kernel, sequence by sequence; f32 rows keep to this one, whose f32 accuracy it lacks
+  uint32_t rows = max_q > (1u << 24) ? 1u << 30 : (max_q ? max_q : 1) * a.group;
+  const bool prompts = dtype != Q4K_F32 && rows > kPromptRows;
+  a.max_rows = prompts ? kPromptRows : 0;
+  const bool all = prompts && a.b.seqs == 1 && a.b.tokens * a.group > kPromptRows;  // no other sequence is left
+  const uint32_t grid = (uint32_t)ctx->sm_count;
+  static_assert(2 * 160 * 16 * (256 + 2) * 4 <= kCtxXfragBytes, "two parts a CTA fit the context's scratch");
+  if (grid > kAttendMaxCtas || (size_t)2 * grid * (a.c.dim == 512 ? 8 : 16) * (a.c.dim + 2) * 4 > ctx->xfrag_cap)
+    return ctx_fail(ctx, Q4K_ERR_UNSUPPORTED, "q4k_paged_attention: %u SMs need more scratch than the context has", grid);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+  if (prompts) {
+    e = launch_prompt(a, dtype, ctx->select.spin_limit, ctx->device, st);
+    if (e != cudaSuccess) return ctx_cuda(ctx, e, "q4k_paged_attention prompt launch");
+    rows = kPromptRows;
+  }
+  if (all) {
+    ctx->err[0] = 0;
+    return Q4K_OK;
+  }
+  if (dtype == Q4K_F32)
+    e = launch_dim<float>(a, rows, grid, ctx->device, st);
+  else if (dtype == Q4K_F16)
+    e = launch_dim<__half>(a, rows, grid, ctx->device, st);
+  else
+    e = launch_dim<__nv_bfloat16>(a, rows, grid, ctx->device, st);
+  return ctx_cuda(ctx, e, "q4k_paged_attention launch");
+}

@@ -1,0 +1,173 @@
+// The paged 8-bit key/value cache: what its kernels share.
+//
+// Codes are e4m3 (4 exponent and 3 mantissa bits), [pages][kv heads][page
+// size][head dim] for keys and for values; each 16 tokens of a page and head
+// (a "block") have one scale, a power of two, [pages][kv heads][page size /
+// 16].  A code stands for code * scale.  Blocks are contiguous (16 * head dim
+// bytes), so a kernel that follows the block table still reads long runs.
+//
+// Why e4m3 with a power of two: an append that raises a block's largest
+// magnitude has to change its scale; with powers of two the codes already
+// there are then only shifted in exponent (exact down to e4m3's subnormals),
+// so a cache filled token by token equals one filled at once, and the scale
+// of a product can be applied to exponents.  Channels much larger than the
+// others, which keys have, cost a floating code nothing.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+#include "q4k_ctx.cuh"
+
+namespace q4k {
+
+constexpr uint32_t kKvBlock = 16;      // tokens under one scale
+constexpr float kCodeMax = 448.0f;     // largest finite e4m3
+constexpr int kScaleExpMin = -60;      // exponents of the block scales
+constexpr int kScaleExpMax = 60;
+
+// Status bits of the context's status word (bit 0: a wait expired, bit 1: a
+// token id past the vocabulary in q4k_ple_stage1).
+constexpr uint32_t kStatusKvMeta = 4u;      // block table, lengths or positions out of range
+constexpr uint32_t kStatusKvNonFinite = 8u; // a key or value was not finite
+constexpr uint32_t kStatusToken = 16u;      // a token id >= V in q4k_token_logprobs
+
+struct KvCache {
+  uint8_t* k;
+  uint8_t* v;
+  float* ks;
+  float* vs;
+  uint32_t pages, page_shift, heads, dim;
+};
+
+struct KvBatch {
+  const uint32_t* table;    // [seqs][cols]
+  const uint32_t* q_start;  // [seqs + 1]
+  const uint32_t* kv_len;   // [seqs], the new tokens included
+  uint32_t seqs, tokens, cols;
+};
+
+// One sequence of a batch, with every value brought into range: `bad` when
+// the caller's were not (the sequence is then treated as empty).
+struct KvSeq {
+  uint32_t t0, n, kv;  // first row, new tokens, tokens in the cache
+  bool bad;
+};
+
+__device__ __forceinline__ KvSeq kv_seq(const KvBatch& bt, uint32_t page_shift, uint32_t b) {
+  KvSeq s;
+  const uint32_t a = bt.q_start[b], e = bt.q_start[b + 1];
+  s.kv = bt.kv_len[b];
+  s.bad = a > e || e > bt.tokens || s.kv > (bt.cols << page_shift);
+  s.t0 = s.bad ? 0 : a;
+  s.n = s.bad ? 0 : e - a;
+  if (s.bad) s.kv = 0;
+  return s;
+}
+
+// Element offset of the block that holds position `pos` (a multiple of 16)
+// of a sequence, in units of blocks: (page * heads + head) * blocks-per-page
+// + block.  64 bits: a cache can hold more than 2^32 codes.  False: the block
+// table's entry is out of range.
+__device__ __forceinline__ bool kv_block(const KvCache& c, uint32_t page, uint32_t head, uint32_t pos,
+                                         uint64_t* block) {
+  const uint32_t per = 1u << (c.page_shift - 4);
+  *block = ((uint64_t)page * c.heads + head) * per + ((pos >> 4) & (per - 1));
+  return page < c.pages;
+}
+
+// The exponent E of a block's scale 2^E: the smallest with amax <= 448 * 2^E,
+// in [kScaleExpMin, kScaleExpMax].  amax finite and >= 0.  448 = 0.875 * 2^9,
+// so with amax = m * 2^e (m in [0.5, 1)) it is e - 9, or e - 8 when m > 0.875.
+__device__ __forceinline__ int kv_scale_exp(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  int e = (int)(u >> 23) - 126;  // subnormal amax: far below the clamp
+  e = (u & 0x7fffffu) > 0x600000u ? e - 8 : e - 9;
+  return min(max(e, kScaleExpMin), kScaleExpMax);
+}
+
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ int exp_of(float pow2) { return (int)((__float_as_uint(pow2) >> 23) & 0xffu) - 127; }
+
+// Two f32 -> two e4m3 codes (lo in the low byte), round to nearest even,
+// saturating at +-448.
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Two e4m3 codes -> f16x2, exact.
+__device__ __forceinline__ uint32_t e4m3_to_f16x2(uint32_t codes16) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)codes16));
+  return r;
+}
+
+// ---- element types of the activations -----------------------------------------
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<float> {
+  static constexpr bool kExact = true;  // results to f32 accuracy
+  static __device__ __forceinline__ float to(float x) { return x; }
+  static __device__ __forceinline__ float from(float x) { return x; }
+};
+template <>
+struct Elem<__half> {
+  static constexpr bool kExact = false;
+  static __device__ __forceinline__ float to(__half x) { return __half2float(x); }
+  static __device__ __forceinline__ __half from(float x) { return __float2half_rn(x); }
+};
+template <>
+struct Elem<__nv_bfloat16> {
+  static constexpr bool kExact = false;
+  static __device__ __forceinline__ float to(__nv_bfloat16 x) { return __bfloat162float(x); }
+  static __device__ __forceinline__ __nv_bfloat16 from(float x) { return __float2bfloat16_rn(x); }
+};
+
+// N consecutive elements, 16-byte aligned, as f32 (N * sizeof(T) a multiple of 16 or equal to 8).
+template <int N, typename T>
+__device__ __forceinline__ void load_elems(const T* p, float (&x)[N]) {
+  constexpr int kBytes = N * sizeof(T);
+  if constexpr (kBytes >= 16) {
+    uint4 w[kBytes / 16];
+#pragma unroll
+    for (int i = 0; i < kBytes / 16; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+    const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = Elem<T>::to(e[i]);
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = Elem<T>::to(e[i]);
+  }
+}
+
+template <int N, typename T>
+__device__ __forceinline__ void store_elems(T* p, const float (&x)[N]) {
+  constexpr int kBytes = N * sizeof(T);
+  alignas(16) T e[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = Elem<T>::from(x[i]);
+  if constexpr (kBytes >= 16) {
+#pragma unroll
+    for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(e)[i];
+  } else {
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(e);
+  }
+}
+
+// Host: the views of the C ABI's structs, checked (kv_append.cu).
+int kv_views(q4k_ctx* ctx, const char* what, const q4k_kv_cache* cache, const q4k_kv_batch* batch, uint32_t dtype,
+             uint32_t q_heads, KvCache* c, KvBatch* b);
+inline size_t dtype_bytes(uint32_t dtype) { return dtype == Q4K_F32 ? 4 : 2; }
+// Rows of `heads * dim` elements `stride` elements apart: 16-byte aligned and not overlapping.
+inline bool rows_ok(const void* p, uint64_t stride, uint64_t row, uint32_t dtype) {
+  return aligned16(p) && (stride * dtype_bytes(dtype)) % 16 == 0 && stride >= row;
+}
+
+}  // namespace q4k

@@ -1,0 +1,475 @@
+// q4k_paged_attention for many rows per sequence (prompts): attention over
+// the paged 8-bit cache (kv_cache.cuh) on the 5th-generation tensor cores.
+// The reference feeds prompts token by token (src/engine.ts:1932-1934).
+//
+// Mathematics as in kv_attend.cu: t_j = s_j + e_j (base-2 score plus the value
+// block's exponent), p_j = 2^(t_j - m), O = sum p_j code_j, l = sum p_j 2^-e_j.
+// The reference m of a row moves only when t exceeds it by 8 (p then stays
+// below 2^8, and f16 holds p * 2^7), so the accumulators are rarely rescaled.
+//
+// Work.  A CTA takes 128 * kTiles rows of one sequence and key head (rows:
+// token-major, the query heads of the key head within, so the heads share
+// every key tile) against the sequence's keys in tiles of 128.  Both products
+// are tcgen05.mma kind::f16 with M = 128: S = Q K^T with both operands in
+// shared memory, O += P V with P in tensor memory.  f16 holds every e4m3 code
+// and every f16 or bf16 row (after a power of two per row) exactly; P is
+// rounded once to f16's 11 bits.
+//   warps 0 .. 4 kTiles - 1   softmax, one thread a row: S from tensor memory,
+//                             statistics, P back over S
+//   the next 4                read codes through the block table, convert them
+//                             to f16 and store them as swizzled operand chunks
+//                             (128 keys x 128 dims) in a ring
+//   the last                  one thread issues the MMAs
+// Tensor memory: two score slots of 128 columns (one per tile, or the two
+// halves of a double buffer when kTiles = 1) and O.  While one slot's softmax
+// runs, the tensor cores work for the other.  Head dims up to 128 run two
+// tiles, so a converted chunk serves 256 rows; 256 one, as O takes half of
+// tensor memory; at 512 a CTA computes half of O's columns and S is computed
+// by both halves (Q alone takes 128 KB of shared memory).
+//
+// Every wait is bounded; on expiry the role records it and returns.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "kv_attend.cuh"
+#include "kv_cache.cuh"
+#include "q4k_ptx.cuh"
+#include "q4k_tcgen05.cuh"
+
+namespace q4k {
+namespace {
+
+constexpr uint32_t kPKeys = 128;        // keys of a tile
+constexpr float kPromptShift = 7.0f;    // P is stored times 2^7
+constexpr float kLazy = 8.0f;           // how far t may exceed the reference
+
+template <int D>
+struct PromptCfg {
+  static constexpr uint32_t kTiles = D <= 128 ? 2 : 1;
+  static constexpr uint32_t kHalves = D == 512 ? 2 : 1;           // CTAs that share a row block, by O's columns
+  static constexpr uint32_t kOut = D / kHalves;                    // O's columns of a CTA
+  static constexpr uint32_t kChunk = D < 128 ? D : 128;            // dims of an operand chunk
+  static constexpr uint32_t kKChunks = D / kChunk, kVChunks = kOut / kChunk;
+  static constexpr uint32_t kChunkBytes = kPKeys * kChunk * 2;
+  static constexpr uint32_t kQBytes = 128 * D * 2;                 // one tile's rows
+  static constexpr uint32_t kRing = D == 512 ? 3 : (D == 64 ? 6 : 5);
+  static constexpr uint32_t kWarps = 4 * kTiles + 5;
+  static constexpr size_t kSmem = 1024 + kTiles * kQBytes + kRing * kChunkBytes;
+  static constexpr uint32_t kOCol = 256;                           // first column of O
+};
+
+__device__ __forceinline__ float ex2p(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
+
+// Instruction descriptor, kind::f16: D fp32, A and B f16, A K-major, M = 128;
+// B K-major, or MN-major (its rows in shared memory are the K index).
+__device__ __forceinline__ uint32_t idesc_f16_m128(uint32_t n, bool b_mn) {
+  return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// A wait whose outcome is the same in every lane of the warp.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t spin) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, spin)) != 0;
+}
+
+struct PromptArgs {
+  AttendArgs a;
+  uint32_t spin;
+};
+
+template <int D, typename T>
+__global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(const PromptArgs pa) {
+  using C = PromptCfg<D>;
+  const AttendArgs& a = pa.a;
+  const uint32_t spin = spin_or_default(pa.spin);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* const sq = smem;                             // [kTiles][D / 64][128 rows][128 bytes], swizzled
+  uint8_t* const ring = smem + C::kTiles * C::kQBytes;  // [kRing][kChunk / 64][128 keys][128 bytes], swizzled
+  __shared__ uint64_t full[C::kRing], empty[C::kRing], s_full[2], p_full[2], o_done[C::kTiles];
+  __shared__ uint32_t s_tmem;
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+  const uint32_t G = a.group, RT = 128 * C::kTiles;
+
+  // which sequence: slot q_start[b] * G / RT + b is its first row block, which
+  // leaves room for a ragged last one; the last blocks (most keys) start first
+  const uint32_t slot = gridDim.x - 1 - blockIdx.x;
+  const uint32_t h = blockIdx.y / C::kHalves, half = blockIdx.y % C::kHalves;
+  uint32_t b = 0;
+  for (uint32_t i0 = 0; i0 < a.b.seqs; i0 += blockDim.x) {
+    const uint32_t i = i0 + tid;
+    b += __syncthreads_count(i < a.b.seqs && (uint64_t)a.b.q_start[i] * G / RT + i <= slot);
+  }
+  if (b == 0) return;
+  --b;
+  const KvSeq s = kv_seq(a.b, a.c.page_shift, b);
+  const uint32_t rows = s.n * G;
+  const uint64_t row0_64 = ((uint64_t)slot - ((uint64_t)a.b.q_start[b] * G / RT + b)) * RT;
+  if (s.bad || rows <= a.max_rows || row0_64 >= rows) return;  // served by the other kernel, or nothing
+  const uint32_t row0 = (uint32_t)row0_64, n_rows = min(RT, rows - row0);
+  const int pos0 = (int)s.kv - (int)s.n;
+  const int pos_first = pos0 + (int)(row0 / G), pos_last = pos0 + (int)((row0 + n_rows - 1) / G);
+  // keys the block's rows can see, from a multiple of 16
+  const int low = a.window ? pos_first - (int)a.window + 1 : 0;
+  const uint32_t key0 = low > 0 ? (uint32_t)low & ~15u : 0u;
+  const uint32_t n_tiles = pos_last >= (int)key0 ? ((uint32_t)pos_last - key0) / kPKeys + 1 : 0;
+  const uint32_t* const table = a.b.table + (uint64_t)b * a.b.cols;
+
+  if (tid == 0) {
+    for (uint32_t i = 0; i < C::kRing; ++i) {
+      mbar_init(&full[i], 4);
+      mbar_init(&empty[i], 1);
+    }
+    for (uint32_t i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+    }
+    for (uint32_t i = 0; i < C::kTiles; ++i) mbar_init(&o_done[i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == C::kWarps - 1) tmem_alloc512(&s_tmem);
+
+  // the rows' operand: f16 under a power of two per row, K-major, 128-byte swizzle
+  float row_c = 0.0f;  // what a score is multiplied with, before the key block's scale
+  int row_pos = -1;
+  const uint32_t group = warp / 4, r = tid & 127u;
+  if (warp < 4 * C::kTiles) {
+    const uint32_t rr = row0 + group * 128 + r;
+    const bool live = group * 128 + r < n_rows;
+    const T* src = static_cast<const T*>(a.q) + (uint64_t)(s.t0 + (live ? rr / G : 0)) * a.q_stride +
+                   (h * G + (live ? rr % G : 0)) * D;
+    float mx = 0.0f;
+    if (live) {
+      row_pos = pos0 + (int)(rr / G);
+      for (uint32_t d = 0; d < (uint32_t)D; d += 8) {
+        float x[8];
+        load_elems(src + d, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (fabsf(x[i]) <= 3.402823466e38f) mx = fmaxf(mx, fabsf(x[i]));
+      }
+    }
+    int e = 13 - ((int)(__float_as_uint(mx) >> 23) - 127);
+    e = mx == 0.0f ? 0 : min(max(e, -110), 110);
+    const float up = a.scale_log2 < 0.0f ? -exp2i(e) : exp2i(e);
+    row_c = fabsf(a.scale_log2) * exp2i(-e);
+    uint8_t* const dst = sq + group * C::kQBytes + r * 128;
+    for (uint32_t d = 0; d < (uint32_t)D; d += 8) {
+      float x[8] = {};
+      if (live) load_elems(src + d, x);
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __half2 hh = __floats2half2_rn(x[2 * i] * up, x[2 * i + 1] * up);
+        w[i] = *reinterpret_cast<const uint32_t*>(&hh);
+      }
+      *reinterpret_cast<uint4*>(dst + (d / 64) * 16384 + ((((d % 64) / 8) ^ (r & 7u)) << 4)) =
+          make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  bool failed = false;
+
+  if (warp < 4 * C::kTiles) {
+    // ---- softmax: this thread's row --------------------------------------------
+    const uint32_t lane_off = (32u * (warp & 3u)) << 16;
+    const uint32_t o_col = tmem + lane_off + C::kOCol + group * C::kOut;
+    const int tile_first = pos0 + (int)((row0 + group * 128) / G);  // the positions of this tile's rows
+    const int tile_last = pos0 + (int)(min(row0 + group * 128 + 127, rows - 1) / G);
+    // lane l < 8: the key scale of the tile's block l; l < 16: the value scale of block l - 8
+    auto scale_of = [&](uint32_t j) {
+      const uint32_t pos = key0 + j * kPKeys + 16 * (lane & 7u);
+      float v = 1.0f;
+      if (lane < 16 && pos < s.kv) {
+        uint64_t blk;
+        if (kv_block(a.c, table[pos >> a.c.page_shift], h, pos, &blk)) v = (lane < 8 ? a.c.ks : a.c.vs)[blk];
+      }
+      return lane < 8 ? v : (float)exp_of(v);
+    };
+    float m = ninf(), l = 0.0f;
+    float sc_next = n_tiles ? scale_of(0) : 0.0f;
+    for (uint32_t j = 0; j < n_tiles; ++j) {
+      const uint32_t u = C::kTiles == 2 ? 2 * j + group : j, sl = u & 1u;
+      const uint32_t s_col = tmem + lane_off + sl * 128;
+      const float sc = sc_next;
+      if (j + 1 < n_tiles) sc_next = scale_of(j + 1);
+      // S of step u was issued after the product of step u - 2, and commits
+      // arrive in their order: o_done is then at most one phase behind j, so
+      // that its parity tells the phase of tile j - 1 below
+      if (!warp_wait(&s_full[sl], (u >> 1) & 1u, spin)) {
+        failed = true;
+        break;
+      }
+      tc_fence_after();
+      const int k0 = (int)(key0 + j * kPKeys);
+      const bool edge = k0 + (int)kPKeys - 1 > tile_first || (a.window && k0 <= tile_last - (int)a.window);
+      const int last = row_pos - k0, first = a.window ? last - (int)a.window + 1 : -1;  // columns first..last are seen
+
+      float top = ninf();
+#pragma unroll
+      for (uint32_t c = 0; c < 4; ++c) {
+        float v[32];
+        tmem_ld32(s_col + 32 * c, v);
+#pragma unroll
+        for (uint32_t k = 0; k < 2; ++k) {
+          if (edge) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int col = (int)(32 * c + 16 * k) + i;
+              if (col > last || col < first) v[16 * k + i] = ninf();
+            }
+          }
+          float bm = v[16 * k];
+#pragma unroll
+          for (int i = 1; i < 16; ++i) bm = fmaxf(bm, v[16 * k + i]);
+          const float ks = __shfl_sync(0xffffffffu, sc, 2 * c + k), ev = __shfl_sync(0xffffffffu, sc, 8 + 2 * c + k);
+          top = fmaxf(top, bm == ninf() ? ninf() : fmaf(bm, ks * row_c, ev));
+        }
+      }
+      // move the reference when the new maximum is far above it
+      const bool move = top > m + kLazy || (m == ninf() && top > ninf());
+      if (__any_sync(0xffffffffu, move)) {
+        const float mn = move ? top : m;
+        const float corr = move && m > ninf() ? ex2p(m - mn) : 1.0f;
+        if (j > 0 && __any_sync(0xffffffffu, corr != 1.0f)) {
+          if (!warp_wait(&o_done[group], (j - 1) & 1u, spin)) {
+            failed = true;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll 1
+          for (uint32_t c = 0; c < C::kOut; c += 16) {
+            float o[16];
+            tmem_ld16(o_col + c, o);
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(o[i] * corr);
+            tmem_st16(o_col + c, w);
+          }
+          tmem_wait_st();
+        }
+        l *= corr;
+        m = mn;
+      }
+      const float ref = m == ninf() ? 0.0f : m - kPromptShift;
+#pragma unroll
+      for (uint32_t c = 0; c < 4; ++c) {
+        float v[32];
+        tmem_ld32(s_col + 32 * c, v);
+        uint32_t w[16];
+#pragma unroll
+        for (uint32_t k = 0; k < 2; ++k) {
+          const float ks = __shfl_sync(0xffffffffu, sc, 2 * c + k), ev = __shfl_sync(0xffffffffu, sc, 8 + 2 * c + k);
+          const float cs = ks * row_c, off = ev - ref;
+          float sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            float x = fmaf(v[16 * k + i], cs, off), y = fmaf(v[16 * k + i + 1], cs, off);
+            if (edge) {
+              const int col = (int)(32 * c + 16 * k) + i;
+              if (col > last || col < first) x = ninf();
+              if (col + 1 > last || col + 1 < first) y = ninf();
+            }
+            x = ex2p(x);
+            y = ex2p(y);
+            sum += x + y;
+            const __half2 hh = __floats2half2_rn(x, y);
+            w[8 * k + i / 2] = *reinterpret_cast<const uint32_t*>(&hh);
+          }
+          l = fmaf(sum, exp2i(-(int)ev), l);
+        }
+        tmem_st16(s_col + 16 * c, w);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[sl]);
+    }
+    // ---- the row's output ---------------------------------------------------------
+    if (!failed && n_tiles && !warp_wait(&o_done[group], (n_tiles - 1) & 1u, spin)) failed = true;
+    tc_fence_after();
+    const bool live = group * 128 + r < n_rows;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // nothing seen: zero; NaN stays
+    const uint32_t rr = row0 + group * 128 + r;
+    T* const dst = static_cast<T*>(a.out) + (uint64_t)(s.t0 + (live ? rr / G : 0)) * a.out_stride +
+                   (h * G + (live ? rr % G : 0)) * D + half * C::kOut;
+    for (uint32_t c = 0; c < C::kOut; c += 16) {
+      float o[16];
+      if (n_tiles && !failed) {
+        tmem_ld16(o_col + c, o);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i] = l != 0.0f ? o[i] * inv : 0.0f;
+      if (live) store_elems(dst + c, o);
+    }
+  } else if (warp < 4 * C::kTiles + 4) {
+    // ---- codes -> f16 operand chunks --------------------------------------------------
+    constexpr uint32_t kLanes = C::kChunk / 16;   // lanes of a row's 16-byte pieces
+    constexpr uint32_t kRowsIt = 32 / kLanes;     // rows a load instruction of a warp covers
+    constexpr uint32_t kIts = 32 / kRowsIt;       // a warp converts 32 of the tile's 128 keys
+    const uint32_t cw = warp - 4 * C::kTiles, x = lane % kLanes, rsub = lane / kLanes;
+    uint32_t seq = 0;
+    bool meta_bad = false;
+    auto fill = [&](bool is_v, uint32_t j, uint32_t chunk) {
+      const uint32_t pos_w = key0 + j * kPKeys + cw * 32;  // the warp's first key, a multiple of 16
+      const uint32_t d0 = (is_v ? half * C::kOut : 0) + chunk * C::kChunk + 16 * x;
+      const uint8_t* base[2];
+#pragma unroll
+      for (uint32_t k = 0; k < 2; ++k) {
+        const uint32_t pos = pos_w + 16 * k;
+        base[k] = nullptr;
+        if (pos < s.kv) {
+          uint64_t blk;
+          if (kv_block(a.c, table[pos >> a.c.page_shift], h, pos, &blk))
+            base[k] = (is_v ? a.c.v : a.c.k) + blk * (16 * D) + d0;
+          else
+            meta_bad = true;
+        }
+      }
+      uint4 code[kIts];
+#pragma unroll
+      for (uint32_t i = 0; i < kIts; ++i) {
+        const uint32_t row = i * kRowsIt + rsub;  // of the warp's 32; block row / 16
+        code[i] = make_uint4(0, 0, 0, 0);
+        const uint8_t* p = base[i * kRowsIt / 16];
+        if (p != nullptr && pos_w + row < s.kv)  // slots past the end are zeros, whatever they hold
+          code[i] = __ldg(reinterpret_cast<const uint4*>(p + (row & 15u) * D));
+      }
+      const uint32_t st = seq % C::kRing, use = seq / C::kRing;
+      if (use > 0 && !warp_wait(&empty[st], (use - 1) & 1u, spin)) {
+        failed = true;
+        return;
+      }
+      uint8_t* const dst = ring + st * C::kChunkBytes + (x / 4) * 16384;
+#pragma unroll
+      for (uint32_t i = 0; i < kIts; ++i) {
+        const uint32_t row = cw * 32 + i * kRowsIt + rsub;
+        const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
+        uint4 o[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          o[k] = make_uint4(e4m3_to_f16x2(w[2 * k] & 0xffffu), e4m3_to_f16x2(w[2 * k] >> 16),
+                            e4m3_to_f16x2(w[2 * k + 1] & 0xffffu), e4m3_to_f16x2(w[2 * k + 1] >> 16));
+        // lanes of the second 64 dims store their pieces in the other order: no bank conflict with the first's
+        const uint32_t c = 2 * (x & 3u), f = (x >> 2) & 1u;
+        *reinterpret_cast<uint4*>(dst + row * 128 + (((c + f) ^ (row & 7u)) << 4)) = f ? o[1] : o[0];
+        *reinterpret_cast<uint4*>(dst + row * 128 + (((c + 1 - f) ^ (row & 7u)) << 4)) = f ? o[0] : o[1];
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[st]);
+      ++seq;
+    };
+    // in the order the MMAs take them
+    if (n_tiles) {
+      for (uint32_t c = 0; c < C::kKChunks && !failed; ++c) fill(false, 0, c);
+      for (uint32_t j = 0; j < n_tiles && !failed; ++j) {
+        if (C::kTiles == 2)
+          for (uint32_t c = 0; c < C::kVChunks && !failed; ++c) fill(true, j, c);
+        if (j + 1 < n_tiles)
+          for (uint32_t c = 0; c < C::kKChunks && !failed; ++c) fill(false, j + 1, c);
+        if (C::kTiles == 1)
+          for (uint32_t c = 0; c < C::kVChunks && !failed; ++c) fill(true, j, c);
+      }
+    }
+    if (__any_sync(0xffffffffu, meta_bad) && lane == 0) atomicOr(a.status, kStatusKvMeta);
+  } else if (lane == 0 && n_tiles) {
+    // ---- MMA issue ------------------------------------------------------------------
+    const uint32_t steps = n_tiles * C::kTiles;
+    const uint32_t id_s = idesc_f16_m128(kPKeys, false), id_o = idesc_f16_m128(C::kChunk, true);
+    const uint64_t dq = smem_desc(smem_u32(sq), 1024, 2), dk = smem_desc(smem_u32(ring), 1024, 2);
+    const uint64_t dv = smem_desc(smem_u32(ring), 1024, 2, 16384);  // the same bytes, keys as the K index
+    uint32_t seq = 0, k_seq = 0, v_seq = 0;  // chunks taken; first chunk of the current key and value tiles
+    auto scores = [&](uint32_t u) {
+      const uint32_t tile = u % C::kTiles;
+      if (tile == 0) k_seq = seq, seq += C::kKChunks;
+      for (uint32_t c = 0; c < C::kKChunks; ++c) {
+        const uint32_t st = (k_seq + c) % C::kRing;
+        if (tile == 0 && !mbar_wait(&full[st], ((k_seq + c) / C::kRing) & 1u, spin)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (uint32_t kk = 0; kk < C::kChunk / 16; ++kk)
+          umma_f16(tmem + (u & 1u) * 128,
+                      dq + (tile * C::kQBytes + (c * (C::kChunk / 64) + kk / 4) * 16384 + (kk % 4) * 32) / 16,
+                      dk + (st * C::kChunkBytes + (kk / 4) * 16384 + (kk % 4) * 32) / 16, id_s, c + kk > 0);
+        if (tile == C::kTiles - 1) umma_commit(&empty[st]);
+      }
+      umma_commit(&s_full[u & 1u]);
+      return true;
+    };
+    auto values = [&](uint32_t u) {
+      const uint32_t tile = u % C::kTiles, j = u / C::kTiles;
+      if (!mbar_wait(&p_full[u & 1u], (u >> 1) & 1u, spin)) return false;
+      tc_fence_after();
+      if (tile == 0) v_seq = seq, seq += C::kVChunks;
+      for (uint32_t c = 0; c < C::kVChunks; ++c) {
+        const uint32_t st = (v_seq + c) % C::kRing;
+        if (tile == 0 && !mbar_wait(&full[st], ((v_seq + c) / C::kRing) & 1u, spin)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (uint32_t kk = 0; kk < kPKeys / 16; ++kk)
+          umma_f16_ts(tmem + C::kOCol + tile * C::kOut + c * C::kChunk, tmem + (u & 1u) * 128 + kk * 8,
+                          dv + (st * C::kChunkBytes + kk * 2048) / 16, id_o, j > 0 || kk > 0);
+        if (tile == C::kTiles - 1) umma_commit(&empty[st]);
+      }
+      umma_commit(&o_done[tile]);
+      return true;
+    };
+    bool ok = scores(0);
+    if (ok && steps > 1) ok = scores(1);
+    for (uint32_t u = 0; u < steps && ok; ++u) {
+      ok = values(u);
+      if (ok && u + 2 < steps) ok = scores(u + 2);
+    }
+    failed = !ok;
+  }
+  if (failed) atomicOr(a.status, 1u);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == C::kWarps - 1) {
+    tc_fence_after();
+    tmem_free512(tmem);
+  }
+}
+
+template <int D, typename T>
+cudaError_t launch(const PromptArgs& pa, int device, cudaStream_t s) {
+  using C = PromptCfg<D>;
+  static std::atomic<uint8_t> attr_set[kAttrDevices];
+  const cudaError_t e = smem_attr_once(attr_set, device, prompt_kernel<D, T>, (int)C::kSmem);
+  if (e != cudaSuccess) return e;
+  const uint32_t rt = 128 * C::kTiles;
+  const uint32_t slots = (uint32_t)(((uint64_t)pa.a.b.tokens * pa.a.group) / rt) + pa.a.b.seqs;
+  prompt_kernel<D, T><<<dim3(slots, pa.a.c.heads * C::kHalves), C::kWarps * 32, C::kSmem, s>>>(pa);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_dim(const PromptArgs& pa, int device, cudaStream_t s) {
+  switch (pa.a.c.dim) {
+    case 64: return launch<64, T>(pa, device, s);
+    case 128: return launch<128, T>(pa, device, s);
+    case 256: return launch<256, T>(pa, device, s);
+    default: return launch<512, T>(pa, device, s);
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_prompt(const AttendArgs& a, uint32_t dtype, uint32_t spin, int device, cudaStream_t s) {
+  const PromptArgs pa{a, spin};
+  return dtype == Q4K_F16 ? launch_dim<__half>(pa, device, s) : launch_dim<__nv_bfloat16>(pa, device, s);
+}
+
+}  // namespace q4k

@@ -4,6 +4,7 @@
 #include <stdint.h>
 #include <string.h>
 
+#include "kv_cache.cuh"
 #include "q4k_ctx.cuh"
 
 using namespace q4k;
@@ -110,7 +111,7 @@ int q4k_create(int device, q4k_ctx** out) {
   const size_t sel_bytes = 256 * sizeof(unsigned long long) + 256;
   const size_t scale_bytes = kCtxScaleSlots * sizeof(float);
   const size_t rows_bytes = kMaxSelectRows * 256 * sizeof(unsigned long long) + 256;
-  const size_t total = sel_bytes + scale_bytes + kCtxXfragBytes + rows_bytes;
+  const size_t total = sel_bytes + scale_bytes + kCtxXfragBytes + rows_bytes + kSplitCounters * sizeof(uint32_t);
   if (cudaMalloc(&ctx->scratch, total) != cudaSuccess) {
     delete ctx;
     return Q4K_ERR_CUDA;
@@ -124,7 +125,9 @@ int q4k_create(int device, q4k_ctx** out) {
   ctx->xfrag_cap = kCtxXfragBytes;
   ctx->row_slots = reinterpret_cast<unsigned long long*>(base + sel_bytes + scale_bytes + kCtxXfragBytes);
   ctx->row_counters = reinterpret_cast<uint32_t*>(ctx->row_slots + kMaxSelectRows * 256);
+  ctx->split_counters = reinterpret_cast<uint32_t*>(base + sel_bytes + scale_bytes + kCtxXfragBytes + rows_bytes);
   if (init_select_scratch(ctx->select, nullptr) != cudaSuccess ||
+      cudaMemsetAsync(ctx->split_counters, 0, kSplitCounters * sizeof(uint32_t), nullptr) != cudaSuccess ||
       init_row_slots(ctx->row_slots, ctx->row_counters, kMaxSelectRows, nullptr) != cudaSuccess ||
       cudaDeviceSynchronize() != cudaSuccess) {
     cudaFree(ctx->scratch);
@@ -164,6 +167,14 @@ int q4k_check(q4k_ctx* ctx) {
       return ctx_fail(ctx, Q4K_ERR_TIMEOUT,
                       "a kernel gave up a bounded wait (its weight copies, a K-split partner or a peer rank's "
                       "candidates did not arrive within the wait limit); its outputs are invalid");
+    if (status & kStatusKvMeta)
+      return ctx_fail(ctx, Q4K_ERR_INVALID_ARG,
+                      "a sequence's rows, length, positions or block table were out of range in a cache call; it was "
+                      "skipped");
+    if (status & kStatusKvNonFinite)
+      return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "a key or value given to q4k_kv_append was not finite");
+    if (status & kStatusToken)
+      return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "a token id was >= V in q4k_token_logprobs; its log probability is NaN");
     return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "a token id was >= vocab in q4k_ple_stage1; that token's outputs are NaN");
   }
   ctx->err[0] = 0;

@@ -20,6 +20,7 @@ struct q4k_ctx {
   float* inv_scale = nullptr;  // [kCtxScaleSlots]: 1/scale per activation row
   unsigned long long* row_slots = nullptr;  // [kMaxSelectRows][256]: q4k_select_rows keys
   uint32_t* row_counters = nullptr;         // [kMaxSelectRows]
+  uint32_t* split_counters = nullptr;       // [kSplitCounters]: arrivals of split rows and segments, 0 between calls
   void* scratch = nullptr;     // the one allocation holding all of the above
   char err[512] = {0};
 };
@@ -30,6 +31,10 @@ namespace q4k {
 // activation rows one single call prepares at most (per-row scales).
 constexpr size_t kCtxXfragBytes = 16u << 20;
 constexpr uint32_t kCtxScaleSlots = 1024;
+
+// Arrival counters of work that several CTAs finish together (attention over
+// a long cache, rows of logits): the last one to arrive merges and resets.
+constexpr uint32_t kSplitCounters = 4096;
 
 inline int ctx_fail(q4k_ctx* ctx, int code, const char* fmt, ...) {
   if (ctx) {

@@ -63,6 +63,68 @@ class Selection:
         return out
 
 
+KV_BLOCK = 16  # tokens under one scale of the 8-bit cache
+KV_HEAD_DIMS = (64, 128, 256, 512)
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # Q4K_F32, Q4K_F16, Q4K_BF16
+
+
+class _KVCacheStruct(ctypes.Structure):  # q4k_kv_cache
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("pages", ctypes.c_uint32), ("page_size", ctypes.c_uint32),
+                ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32)]
+
+
+class _KVBatchStruct(ctypes.Structure):  # q4k_kv_batch
+    _fields_ = [("block_table", ctypes.c_void_p), ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+                ("seqs", ctypes.c_uint32), ("tokens", ctypes.c_uint32), ("table_cols", ctypes.c_uint32)]
+
+
+class KVCache:
+    """A paged 8-bit key/value cache (q4k_kv_cache): e4m3 codes k, v
+    [pages, kv_heads, page_size, head_dim] and power-of-two scales k_scale,
+    v_scale f32 [pages, kv_heads, page_size / 16]; a code stands for
+    code * scale.  Made once; the calls that use it check only their batch."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        if not isinstance(k, torch.Tensor) or k.dim() != 4:
+            raise ValueError("k must be [pages, kv_heads, page_size, head_dim]")
+        pages, heads, page, dim = k.shape
+        for t, name in ((k, "k"), (v, "v")):
+            _need(t, torch.float8_e4m3fn, name, k.device)
+            if t.shape != k.shape:
+                raise ValueError("k and v differ in shape")
+        if page % KV_BLOCK or page & (page - 1):
+            raise ValueError(f"page_size={page} is not a power of two and a multiple of {KV_BLOCK}")
+        if dim not in KV_HEAD_DIMS:
+            raise ValueError(f"head_dim={dim} is not one of {KV_HEAD_DIMS}")
+        for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            _need(t, torch.float32, name, k.device)
+            if tuple(t.shape) != (pages, heads, page // KV_BLOCK):
+                raise ValueError(f"{name} must be [pages, kv_heads, page_size / {KV_BLOCK}]")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, page, dim
+        self.device = k.device
+        self._struct = _KVCacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, page,
+                                      heads, dim)
+        self._ref = ctypes.byref(self._struct)
+
+    @classmethod
+    def allocate(cls, pages: int, kv_heads: int, page_size: int, head_dim: int,
+                 device: int | torch.device = 0) -> "KVCache":
+        """An empty cache (zero codes)."""
+        dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        code = dict(dtype=torch.uint8, device=dev)
+        k, v = (torch.zeros((pages, kv_heads, page_size, head_dim), **code).view(torch.float8_e4m3fn)
+                for _ in range(2))
+        ks, vs = (torch.ones((pages, kv_heads, page_size // KV_BLOCK), dtype=torch.float32, device=dev)
+                  for _ in range(2))
+        return cls(k, v, ks, vs)
+
+    def bytes_per_token(self) -> float:
+        """Codes and scales of one token, keys and values of every head."""
+        return 2 * self.kv_heads * (self.head_dim + 4 / KV_BLOCK)
+
+
 class Context:
     """A libq4k context on one CUDA device (q4k_create / q4k_destroy)."""
 
@@ -366,6 +428,133 @@ class Context:
             self._h, _ptr(weight), _ptr(x), V, N, cap, row_offset, _ptr(out.logits), _ptr(out.cand_val),
             _ptr(out.cand_idx), _ptr(out.argmax), _stream(stream)))
         return out
+
+    # ---- cached attention (see include/q4k.h) ----------------------------------
+
+    def _rows(self, t: torch.Tensor, name: str, dtype: torch.dtype, tokens: int, dim: int) -> tuple[int, int]:
+        """(heads, row stride) of rows [tokens, heads, head_dim]: any row stride, heads side by side."""
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if t.device != self.device:
+            raise ValueError(f"{name} is on {t.device}, expected {self.device}")
+        if t.dtype != dtype:
+            raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
+        shape, stride = t.shape, t.stride()
+        if len(shape) != 3 or shape[0] != tokens or shape[2] != dim:
+            raise ValueError(f"{name} must be [{tokens}, heads, {dim}]")
+        if stride[2] != 1 or (stride[1] != dim and shape[1] > 1):
+            raise ValueError(f"{name}: the heads of a row must be contiguous")
+        return shape[1], stride[0] if tokens > 1 else shape[1] * dim
+
+    def _batch(self, cache: KVCache, tokens: int, block_table: torch.Tensor, q_start: torch.Tensor,
+               kv_len: torch.Tensor):
+        if not isinstance(cache, KVCache):
+            raise TypeError("cache must be a KVCache")
+        if cache.device != self.device:
+            raise ValueError(f"cache is on {cache.device}, expected {self.device}")
+        _need(block_table, torch.int32, "block_table", self.device)
+        _need(q_start, torch.int32, "q_start", self.device)
+        _need(kv_len, torch.int32, "kv_len", self.device)
+        seqs = kv_len.numel()
+        if block_table.dim() != 2 or block_table.shape[0] != seqs or q_start.numel() != seqs + 1:
+            raise ValueError("block_table must be [seqs, columns], q_start [seqs + 1] and kv_len [seqs]")
+        return ctypes.byref(_KVBatchStruct(block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), seqs, tokens,
+                                           block_table.shape[1]))
+
+    def kv_append(self, cache: KVCache, k: torch.Tensor, v: torch.Tensor, rope: torch.Tensor | None,
+                  block_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
+                  q: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+                  stream: torch.cuda.Stream | None = None) -> torch.Tensor | None:
+        """Append new keys and values [tokens, kv_heads, head_dim] to the paged
+        8-bit cache, keys rotated by their positions on the way
+        (q4k_kv_append).  rope: f32 [positions, pairs, 2] of (cos, sin), or
+        None for no rotation.  kv_len counts the new tokens.  With q
+        [tokens, q_heads, head_dim] the queries are rotated in the same launch
+        and returned (q_out, which may be q)."""
+        tokens, dim, dtype = k.shape[0], cache.head_dim, k.dtype
+        if dtype not in DTYPES:
+            raise TypeError(f"k has dtype {dtype}, expected one of {tuple(DTYPES)}")
+        heads, k_stride = self._rows(k, "k", dtype, tokens, dim)
+        v_heads, v_stride = self._rows(v, "v", dtype, tokens, dim)
+        if heads != cache.kv_heads or v_heads != cache.kv_heads:
+            raise ValueError(f"k and v must have the cache's {cache.kv_heads} heads")
+        rope_len = rope_dim = q_heads = q_stride = qo_stride = 0
+        if rope is not None:
+            _need(rope, torch.float32, "rope", self.device)
+            if rope.dim() != 3 or rope.shape[2] != 2:
+                raise ValueError("rope must be [positions, pairs, 2]")
+            rope_len, rope_dim = rope.shape[0], 2 * rope.shape[1]
+        if q is not None:
+            q_heads, q_stride = self._rows(q, "q", dtype, tokens, dim)
+            if q_out is None:
+                q_out = torch.empty((tokens, q_heads, dim), dtype=dtype, device=self.device)
+            qo_heads, qo_stride = self._rows(q_out, "q_out", dtype, tokens, dim)
+            if qo_heads != q_heads:
+                raise ValueError("q_out and q differ in shape")
+        self._check(self._L.q4k_kv_append(
+            self._h, cache._ref, self._batch(cache, tokens, block_table, q_start, kv_len), DTYPES[dtype], _ptr(k),
+            k_stride, _ptr(v), v_stride, _ptr(rope), rope_len, rope_dim, _ptr(q), q_stride,
+            _ptr(q_out) if q is not None else None, qo_stride, q_heads, _stream(stream)))
+        return q_out if q is not None else None
+
+    def paged_attention(self, cache: KVCache, q: torch.Tensor, block_table: torch.Tensor, q_start: torch.Tensor,
+                        kv_len: torch.Tensor, max_q: int, scale: float, window: int = 0,
+                        out: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+        """Causal attention of q [tokens, q_heads, head_dim] over the paged
+        8-bit cache (q4k_paged_attention): row i of a sequence's n new rows has
+        position kv_len - n + i and sees the positions up to its own, the last
+        `window` of them when window > 0; a row that sees none is zero.  max_q:
+        the most new rows of one sequence, known on the host."""
+        tokens, dim, dtype = q.shape[0], cache.head_dim, q.dtype
+        if dtype not in DTYPES:
+            raise TypeError(f"q has dtype {dtype}, expected one of {tuple(DTYPES)}")
+        heads, q_stride = self._rows(q, "q", dtype, tokens, dim)
+        if window < 0 or max_q < 0:
+            raise ValueError("window and max_q must not be negative")
+        if out is None:
+            out = torch.empty((tokens, heads, dim), dtype=dtype, device=self.device)
+        out_heads, out_stride = self._rows(out, "out", dtype, tokens, dim)
+        if out_heads != heads:
+            raise ValueError("out and q differ in shape")
+        self._check(self._L.q4k_paged_attention(
+            self._h, cache._ref, self._batch(cache, tokens, block_table, q_start, kv_len), DTYPES[dtype], _ptr(q),
+            q_stride, _ptr(out), out_stride, heads, max_q, scale, window, _stream(stream)))
+        return out
+
+    # ---- token log probabilities ---------------------------------------------------
+
+    def token_logprobs(self, logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, cap: float = 0.0,
+                       stream: torch.cuda.Stream | None = None
+                       ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Of each row of logits [rows, V] (f32, f16 or bf16; any row stride),
+        softcapped by `cap` when cap > 0 (q4k_token_logprobs): the log
+        probability of tokens[row] (int32; NaN for a negative one: none asked
+        for), the entropy, and the `top` (0..32) most likely tokens in
+        descending order, ties to the lower index.  Returns (logprob [rows],
+        entropy [rows], top_logprob [rows, top], top_token int32 [rows, top])."""
+        if not isinstance(logits, torch.Tensor):
+            raise TypeError("logits must be a torch.Tensor")
+        if logits.device != self.device:
+            raise ValueError(f"logits is on {logits.device}, expected {self.device}")
+        if logits.dtype not in DTYPES:
+            raise TypeError(f"logits has dtype {logits.dtype}, expected one of {tuple(DTYPES)}")
+        if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+            raise ValueError("logits must be [rows, V] with contiguous rows")
+        _need(tokens, torch.int32, "tokens", self.device)
+        rows, V = logits.shape
+        if tokens.numel() != rows:
+            raise ValueError("tokens must hold one id for each row")
+        if top < 0 or top > min(32, V):
+            raise ValueError("top must lie in 0..32 and not exceed V")
+        stats = torch.empty((2, rows), dtype=torch.float32, device=self.device)
+        top_logprob = torch.empty((rows, top), dtype=torch.float32, device=self.device)
+        top_token = torch.empty((rows, top), dtype=torch.int32, device=self.device)
+        logprob, entropy = stats.unbind(0)
+        self._check(self._L.q4k_token_logprobs(
+            self._h, DTYPES[logits.dtype], _ptr(logits), logits.stride(0) if rows > 1 else V, rows, V, cap,
+            _ptr(tokens), top, _ptr(logprob), _ptr(entropy), _ptr(top_logprob) if top else None,
+            _ptr(top_token) if top else None, _stream(stream)))
+        return logprob, entropy, top_logprob, top_token
 
     def exchange(self, rank: int, world: int) -> "Exchange":
         """A mailbox for the fused sharded LM head (see Exchange)."""

@@ -320,6 +320,98 @@ Q4K_API int q4k_ple_stage1(q4k_ctx* ctx, const void* table_q5k, const uint32_t* 
                            uint32_t vocab, uint32_t layers, const float* projected, const uint16_t* norm_w,
                            float eps, float* out, void* stream);
 
+/* ---- paged 8-bit key/value cache ----------------------------------------
+ * What a decode step needs between its q/k/v products and its o product.
+ * The reference keeps an f32 cache per layer and runs one pass each for the
+ * rotation, the stores, the scores, the softmax and the weighted sum
+ * (shaders/rope.wgsl, kv_cache_store.wgsl, attn_score.wgsl, softmax.wgsl,
+ * attn_output.wgsl; src/engine.ts:1562-1584).  Here keys and values are e4m3
+ * codes in pages that a block table orders, with one power-of-two scale for
+ * each 16 tokens of a page and head: a code stands for code * scale.  No
+ * code at a position that holds a token is ever NaN; slots past the end of a
+ * sequence may hold anything.
+ *
+ * A batch is described on the device: sequence b's new rows are
+ * q_start[b] .. q_start[b+1], and kv_len[b] tokens are in its cache once they
+ * have been appended, so row q_start[b] + i has position
+ * kv_len[b] - (q_start[b+1] - q_start[b]) + i.  Position p of sequence b is
+ * slot p % page_size of page block_table[b][p / page_size].  Several
+ * sequences may share full pages; a page being appended to has one owner.
+ * The device-side values are checked by the kernels: a sequence whose rows,
+ * length or pages are out of range is skipped (its output rows are zero or
+ * left unwritten) and q4k_check returns Q4K_ERR_INVALID_ARG. */
+#define Q4K_F32 0
+#define Q4K_F16 1
+#define Q4K_BF16 2
+
+typedef struct {
+  void* k;             /* e4m3 [pages][kv_heads][page_size][head_dim] */
+  void* v;             /* the same */
+  float* k_scale;      /* [pages][kv_heads][page_size / 16], powers of two */
+  float* v_scale;
+  uint32_t pages;
+  uint32_t page_size;  /* a power of two, 16..1024 */
+  uint32_t kv_heads;
+  uint32_t head_dim;   /* 64, 128, 256 or 512 */
+} q4k_kv_cache;
+
+typedef struct {
+  const uint32_t* block_table; /* [seqs][table_cols] */
+  const uint32_t* q_start;     /* [seqs + 1], not decreasing */
+  const uint32_t* kv_len;      /* [seqs] */
+  uint32_t seqs;               /* at most 65536 */
+  uint32_t tokens;             /* new rows in all (q_start[seqs]), at most 2^24 */
+  uint32_t table_cols;
+} q4k_kv_batch;
+
+/* Append the batch's new keys and values (k, v: rows of kv_heads * head_dim
+ * elements of `dtype`, `*_stride` elements apart) to the cache.  Keys are
+ * rotated by their positions first: pairs (j, j + rope_dim/2) of the first
+ * rope_dim elements of a head by rope[position][j] = (cos, sin), a
+ * [rope_len][rope_dim/2][2] table (rope_dim = 0: no rotation; the pairing of
+ * shaders/rope.wgsl:14-20; store as shaders/kv_cache_store.wgsl).  With q (may
+ * be NULL) the batch's queries, q_heads a row, are rotated into q_out in the
+ * same launch (q_out may be q).  A block's scale is the smallest power of two
+ * that holds its largest magnitude; it grows as tokens arrive and the codes
+ * already there are rescaled, so the order and size of the appends do not
+ * matter (but for e4m3's subnormal range).  Infinities are stored as the
+ * block's largest code and NaN as zero, and q4k_check then returns
+ * Q4K_ERR_INVALID_ARG. */
+Q4K_API int q4k_kv_append(q4k_ctx* ctx, const q4k_kv_cache* cache, const q4k_kv_batch* batch, uint32_t dtype,
+                          const void* k, uint64_t k_stride, const void* v, uint64_t v_stride, const float* rope,
+                          uint32_t rope_len, uint32_t rope_dim, const void* q, uint64_t q_stride, void* q_out,
+                          uint64_t q_out_stride, uint32_t q_heads, void* stream);
+
+/* Causal attention of the batch's rows over the cache: out[r][h] =
+ * sum_j softmax_j(scale * q[r][h] . k[j]) v[j] over the positions j of the
+ * row's sequence up to its own, the last `window` of them when window > 0
+ * (shaders/attn_score.wgsl:14-39, softmax.wgsl, attn_output.wgsl:10-22);
+ * head h reads key head h / (q_heads / kv_heads).  A row that sees no
+ * position is zero.  q, out: rows of q_heads * head_dim elements of `dtype`.
+ * f32 rows are computed to f32 accuracy, f16 and bf16 rows to that of their
+ * type, sums and softmax statistics in f32 for all.  max_q: the largest
+ * number of new rows of one sequence, a hint that selects kernels.  Uses the
+ * context's scratch: order the calls of one context on one stream. */
+Q4K_API int q4k_paged_attention(q4k_ctx* ctx, const q4k_kv_cache* cache, const q4k_kv_batch* batch, uint32_t dtype,
+                                const void* q, uint64_t q_stride, void* out, uint64_t out_stride, uint32_t q_heads,
+                                uint32_t max_q, float scale, uint32_t window, void* stream);
+
+/* For each of `rows` rows of V logits (of `dtype`, `stride` elements apart):
+ * x = cap > 0 ? cap * tanh(logit / cap) : logit (shaders/logit_softcap.wgsl),
+ *   logprob = x[token] - log sum exp x           (NaN for token < 0: none)
+ *   entropy = -sum p log p, p = softmax(x)
+ *   top_token / top_logprob [rows][top]: the `top` (0..32) largest logits in
+ * descending order, ties to the lower index, NaN last, and their
+ * log probabilities.  Sums in f32.  A token >= V gives NaN and q4k_check
+ * returns Q4K_ERR_INVALID_ARG.  A row with a NaN or +inf has NaN statistics;
+ * one with nothing above -inf has log probabilities of -inf and entropy 0.
+ * The reference samples from 256 raw candidates on the host
+ * (src/engine.ts:1792-1837) and has no log probabilities.  Uses the
+ * context's scratch: order the calls of one context on one stream. */
+Q4K_API int q4k_token_logprobs(q4k_ctx* ctx, uint32_t dtype, const void* logits, uint64_t stride, uint32_t rows,
+                               uint32_t V, float cap, const int32_t* tokens, uint32_t top, float* logprob,
+                               float* entropy, float* top_logprob, int32_t* top_token, void* stream);
+
 /* ---- the chained decode step -------------------------------------------
  * One token's layers as a true chain, each layer reading the previous
  * layer's output, in ONE persistent launch (plus the fused LM head): the

@@ -1,0 +1,223 @@
+"""q4k_kv_append on the GPU against the 64-bit restatement.
+
+Bounds.  A rotated element is two products and a sum in f32: off by at most
+3 * 2^-24 of |x_j| + |x_j'|.  A code is its nearest e4m3 value: off by at
+most 2^-4 of the value, or half a subnormal step, 2^-10 of the scale.  Both
+together with 1e-5 of slack for the rotation's error near a tie.  Scales are
+powers of two fixed by the block's largest magnitude: exact, as no test input
+sits within rounding of a boundary.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import kv_reference as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def make(new, past, hq, hkv, d, page, rot, dtype, seed=1):
+    import q4k
+
+    kv = [n + p for n, p in zip(new, past)]
+    pr = R.Problem(new, kv, hq, hkv, d, page, seed=seed)
+    g = torch.Generator().manual_seed(seed + 100)
+    k = (torch.randn(pr.tokens, hkv, d, generator=g) * 3).to(dtype)
+    v = torch.randn(pr.tokens, hkv, d, generator=g).to(dtype)
+    q = torch.randn(pr.tokens, hq, d, generator=g).to(dtype)
+    rope = R.rope_table(max(kv) + 1, rot) if rot else None
+    return q4k, pr, k, v, q, rope
+
+
+def check(pr, cache, k, v, rope, past):
+    """Every code and scale of the cache after the append."""
+    hkv, d, page = pr.hkv, pr.d, pr.page
+    before = {"k": R.dequant(pr.k, pr.k_scale), "v": R.dequant(pr.v, pr.v_scale)}
+    for name, x in (("k", k.double()), ("v", v.double())):
+        codes, scale = getattr(cache, name).cpu(), getattr(cache, name + "_scale").cpu()
+        got = R.dequant(codes, scale)
+        old_scale = getattr(pr, name + "_scale")
+        want, exp_scale = before[name].clone(), old_scale.double().clone()
+        slack = torch.zeros_like(want)
+        for b, n in enumerate(pr.new):
+            for i in range(n):
+                p = past[b] + i
+                pg, slot = int(pr.table[b, p // page]), p % page
+                row = x[pr.q_start[b] + i]
+                if name == "k" and rope is not None:
+                    cs = rope[p].double()
+                    row = R.rotate(row, cs[:, 0].expand(hkv, -1), cs[:, 1].expand(hkv, -1))
+                blk = slot // 16
+                if p % 16 == 0:  # a block that begins now: what it held is gone
+                    exp_scale[pg, :, blk] = 2.0**-60
+                    want[pg, :, slot : slot + 16] = 0
+                want[pg, :, slot] = row
+                exp_scale[pg, :, blk] = torch.maximum(exp_scale[pg, :, blk], R.scale_of(row.abs().amax(-1)))
+        assert torch.equal(scale.double(), exp_scale)
+        step = exp_scale.repeat_interleave(16, -1)[..., None]
+        bound = torch.maximum(want.abs() * 2.0**-4, step * 2.0**-10) + 1e-5 * want.abs().amax()
+        # slots of a fresh block that no token has reached yet keep any code
+        for b, n in enumerate(pr.new):
+            end = past[b] + n
+            if end % 16 and n and end // 16 * 16 >= past[b]:
+                pg, slot = int(pr.table[b, (end - 1) // page]), end % page
+                if slot:
+                    got[pg, :, slot : slot // 16 * 16 + 16] = 0
+                    want[pg, :, slot : slot // 16 * 16 + 16] = 0
+        # codes that were only rescaled or left alone: exact, or half a subnormal step
+        assert ((got - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize(
+    "new,past,hq,hkv,d,page,rot",
+    [
+        ([1], [0], 8, 1, 256, 16, 256),
+        ([1], [37], 8, 1, 256, 16, 256),
+        ([1, 1, 1], [15, 16, 17], 4, 2, 64, 32, 64),
+        ([5, 0, 33, 1, 48], [3, 9, 31, 0, 16], 6, 2, 128, 64, 32),
+        ([100, 7], [250, 0], 3, 3, 512, 128, 128),
+        ([17, 2], [15, 30], 1, 1, 64, 16, 0),
+    ],
+)
+def test_codes_scales_and_queries(ctx, dtype, new, past, hq, hkv, d, page, rot):
+    q4k, pr, k, v, q, rope = make(new, past, hq, hkv, d, page, rot, dtype)
+    cache, _, table, qs, kvl = pr.device(DEV, q4k, dtype)
+    rd = rope.to(DEV) if rope is not None else None
+    out = ctx.kv_append(cache, k.to(DEV), v.to(DEV), rd, table, qs, kvl, q=q.to(DEV)).cpu()
+    ctx.check()
+    check(pr, cache, k, v, rope, past)
+    for b, n in enumerate(new):
+        for i in range(n):
+            t = pr.q_start[b] + i
+            want = q[t].double()
+            if rope is not None:
+                cs = rope[past[b] + i].double()
+                want = R.rotate(want, cs[:, 0].expand(hq, -1), cs[:, 1].expand(hq, -1))
+            tol = {F32: 2.0**-22, F16: 2.0**-11, BF16: 2.0**-8}[dtype]
+            assert ((out[t].double() - want).abs() <= tol * (want.abs() + q[t].double().abs().amax() * 2.0**-10) + (
+                3 * 2.0**-23) * q[t].double().abs().amax()).all()
+
+
+def test_one_by_one_equals_at_once(ctx):
+    """Power-of-two scales: growth only shifts exponents, so the caches agree
+    wherever a code is not subnormal (below 2^-6 of the scale)."""
+    q4k, pr, k, v, q, rope = make([45], [3], 2, 2, 128, 16, 128, F32, seed=5)
+    k = k * torch.logspace(-2, 2, 45)[:, None, None]  # scales that grow on the way
+    rd = rope.to(DEV)
+    cache, _, table, qs, kvl = pr.device(DEV, q4k, F32)
+    ctx.kv_append(cache, k.to(DEV), v.to(DEV), rd, table, qs, kvl)
+    one, _, _, _, _ = pr.device(DEV, q4k, F32)
+    two = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    for i in range(45):
+        ctx.kv_append(one, k[i : i + 1].to(DEV), v[i : i + 1].to(DEV), rd, table, two,
+                      torch.tensor([4 + i], dtype=torch.int32, device=DEV))
+    ctx.check()
+    for name in ("k", "v"):
+        assert torch.equal(getattr(cache, name + "_scale"), getattr(one, name + "_scale"))
+        a, b = (getattr(c, name).cpu().double() for c in (cache, one))
+        normal = a.abs() >= 2.0**-6
+        assert torch.equal(a[normal], b[normal])
+        assert ((a - b).abs() <= 2.0**-9).all()
+
+
+def test_repeat_and_strides(ctx):
+    """Rows out of one packed buffer, q in place, another stream, twice: the same bits."""
+    q4k, pr, k, v, q, rope = make([9, 4], [20, 7], 4, 2, 128, 32, 64, BF16, seed=7)
+    rd = rope.to(DEV)
+    caches = []
+    for packed in (False, True):
+        cache, _, table, qs, kvl = pr.device(DEV, q4k, BF16)
+        kd, vd, qd = k.to(DEV), v.to(DEV), q.to(DEV)
+        if packed:
+            buf = torch.cat([qd.flatten(1), kd.flatten(1), vd.flatten(1)], 1)
+            qd, kd, vd = buf[:, :512].view(-1, 4, 128), buf[:, 512:768].view(-1, 2, 128), buf[:, 768:].view(-1, 2, 128)
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                out = ctx.kv_append(cache, kd, vd, rd, table, qs, kvl, q=qd, q_out=qd)
+            torch.cuda.current_stream().wait_stream(s)
+        else:
+            out = ctx.kv_append(cache, kd, vd, rd, table, qs, kvl, q=qd)
+        caches.append((cache, out.clone()))
+    (a, qa), (b, qb) = caches
+    assert torch.equal(qa, qb)
+    for name in ("k", "v"):
+        assert torch.equal(getattr(a, name).view(torch.uint8), getattr(b, name).view(torch.uint8))
+        assert torch.equal(getattr(a, name + "_scale"), getattr(b, name + "_scale"))
+
+
+def test_not_finite_is_reported_and_contained(ctx):
+    from q4k import Q4KError
+
+    q4k, pr, k, v, q, rope = make([4], [0], 1, 1, 64, 16, 0, F32, seed=9)
+    v[1, 0, 3], v[2, 0, 5], v[3, 0, 7] = float("inf"), float("nan"), float("-inf")
+    cache, _, table, qs, kvl = pr.device(DEV, q4k, F32)
+    ctx.kv_append(cache, k.to(DEV), v.to(DEV), None, table, qs, kvl)
+    with pytest.raises(Q4KError, match="not finite"):
+        ctx.check()
+    ctx.check()  # the record was cleared
+    pg = int(pr.table[0, 0])
+    codes = cache.v.cpu().double()[pg, 0, :4]
+    assert torch.isfinite(codes).all()
+    assert codes[1, 3] == 448 and codes[2, 5] == 0 and codes[3, 7] == -448
+    fin = torch.isfinite(v[:, 0])
+    s = float(cache.v_scale.cpu()[pg, 0, 0])
+    assert s == float(R.scale_of(v[:, 0][fin].double().abs().max()))
+    assert ((codes * s - v[:, 0].double()).abs()[fin] <= torch.maximum(
+        v[:, 0].double().abs()[fin] * 2.0**-4, torch.tensor(s * 2.0**-10))).all()
+
+
+@pytest.mark.parametrize("what", ["page", "length", "rope", "rows"])
+def test_bad_metadata_is_reported_and_skipped(ctx, what):
+    """The kernels check what the host cannot see; the other sequence is served."""
+    from q4k import Q4KError
+
+    q4k, pr, k, v, q, rope = make([3, 2], [5, 20], 2, 1, 64, 16, 64, F32, seed=11)
+    cache, _, table, qs, kvl = pr.device(DEV, q4k, F32)
+    rd = rope.to(DEV)
+    if what == "page":
+        table[0, 0] = pr.pages + 5
+    elif what == "length":
+        kvl[0] = 10_000
+    elif what == "rope":
+        rd = rd[:8].contiguous()  # too short for sequence 1
+    else:
+        qs = torch.tensor([3, 0, 5], dtype=torch.int32, device=DEV)
+    before = cache.k.clone()
+    ctx.kv_append(cache, k.to(DEV), v.to(DEV), rd, table, qs, kvl)
+    with pytest.raises(Q4KError, match="out of range"):
+        ctx.check()
+    good = 1 if what in ("page", "length") else 0
+    if what != "rows":
+        p = (20 if good else 5)
+        pg = int(pr.table[good, p // 16])
+        assert not torch.equal(cache.k[pg].view(torch.uint8), before[pg].view(torch.uint8))
+
+
+def test_refusals(ctx):
+    q4k, pr, k, v, q, rope = make([3], [5], 2, 1, 64, 16, 64, F32)
+    cache, _, table, qs, kvl = pr.device(DEV, q4k, F32)
+    kd, vd, qd, rd = k.to(DEV), v.to(DEV), q.to(DEV), rope.to(DEV)
+    ok = dict(cache=cache, k=kd, v=vd, rope=rd, block_table=table, q_start=qs, kv_len=kvl)
+    bad = [
+        (dict(k=kd.double()), TypeError), (dict(v=vd.half()), TypeError), (dict(k=kd[:, :, :32]), ValueError),
+        (dict(v=vd[:2]), ValueError), (dict(rope=rd[:, :, :1]), ValueError), (dict(rope=rd[:, :5].contiguous()), q4k.Q4KError),
+        (dict(q_start=qs.long()), TypeError), (dict(q_start=qs[:1]), ValueError), (dict(block_table=table[0]), ValueError),
+        (dict(kv_len=kvl.cpu()), ValueError), (dict(cache=None), AttributeError), (dict(q=qd, q_out=qd[:, :1]), ValueError),
+        (dict(k=torch.zeros(3, 1, 65, device=DEV)[:, :, 1:]), q4k.Q4KError),  # rows not 16-byte aligned
+    ]
+    for change, err in bad:
+        with pytest.raises(err):
+            ctx.kv_append(**{**ok, **change})
+    with pytest.raises(ValueError):
+        q4k.KVCache(cache.k, cache.v[:1], cache.k_scale, cache.v_scale)
+    with pytest.raises(ValueError):
+        q4k.KVCache.allocate(2, 1, 24, 64)
+    with pytest.raises(ValueError):
+        q4k.KVCache.allocate(2, 1, 16, 96)
+    ctx.kv_append(**{**ok, "k": kd[:0], "v": vd[:0]})  # nothing to do
+    ctx.check()

@@ -1,0 +1,167 @@
+"""q4k_token_logprobs on the GPU against 64-bit values.
+
+Bounds.  Sums of up to 3e5 positive f32 terms, each off by 2^-22 (the
+exponential) and added in runs of 1e3 and trees: relative 1e-5 at most, so
+lse is off by 1e-5 besides its own rounding, |lse| * 2^-23; a softcapped logit
+by 4 * 2^-23 of the cap.  The entropy's weighted sum alike, times its size.
+Alternatives are whole numbers: equal.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def reference(logits, tokens, top, cap):
+    raw = logits.double()
+    x = torch.tanh(raw / cap) * cap if cap > 0 else raw
+    lse = torch.logsumexp(x, 1, keepdim=True)
+    logp = x - lse
+    p = logp.exp()
+    ent = -torch.where(p > 0, p * logp, torch.zeros_like(p)).sum(1)
+    order = torch.sort(raw + 0.0, dim=1, descending=True, stable=True).indices[:, :top]
+    return logp.gather(1, tokens.long().clamp(min=0)[:, None])[:, 0], ent, logp.gather(1, order), order
+
+
+def check(ctx, logits, tokens, top, cap=0.0):
+    lp, ent, tl, ti = (t.cpu() for t in ctx.token_logprobs(logits.to(DEV), tokens.to(DEV), top=top, cap=cap))
+    ctx.check()
+    wl, we, wt, wi = reference(logits, tokens, top, cap)
+    finite = logits.double().abs()[torch.isfinite(logits)]
+    size = 2e-5 * (1 + finite.amax().clamp(max=cap if cap > 0 else math.inf))
+
+    def near(a, b):  # equal infinities, or within the bound
+        return bool(((a.double() == b) | ((a.double() - b).abs() <= size)).all())
+
+    assert near(lp, wl)
+    assert ((ent.double() - we).abs() <= 2e-5 * (1 + we.abs()) * 2).all()
+    assert torch.equal(ti.long(), wi)
+    assert near(tl, wt)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("rows,V,top", [(1, 1, 1), (1, 7, 7), (3, 33, 32), (2, 1000, 5), (5, 4096, 20), (4, 4099, 20),
+                                        (2, 50001, 32), (700, 2053, 3), (1, 262144, 20), (3, 9000, 0)])
+def test_against_64_bits(ctx, dtype, cap, rows, V, top):
+    g = torch.Generator().manual_seed(V + rows)
+    logits = (torch.randn(rows, V, generator=g) * 4).to(dtype)
+    tokens = torch.randint(0, V, (rows,), generator=g, dtype=torch.int32)
+    check(ctx, logits, tokens, top, cap)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [300, 5000, 60000])
+def test_ties_go_to_the_lowest_index(ctx, dtype, V):
+    g = torch.Generator().manual_seed(V)
+    rows = [torch.zeros(V), torch.randint(0, 3, (V,), generator=g).float(), torch.zeros(V), torch.zeros(V)]
+    rows[2][V // 2 :: 7] = 1.0
+    rows[3][::2] = -0.0  # equal to +0
+    check(ctx, torch.stack(rows).to(dtype), torch.tensor([0, V - 1, V // 2, 1], dtype=torch.int32), 20)
+
+
+@pytest.mark.parametrize("V", [200, 9000, 70000])
+def test_ascending_and_descending(ctx, V):
+    """Every tile brings better ones, or none does."""
+    up = torch.arange(V, dtype=F32) / V * 20
+    check(ctx, torch.stack([up, up.flip(0)]), torch.tensor([3, 5], dtype=torch.int32), 32)
+
+
+@pytest.mark.parametrize("V,rows", [(40, 2), (9000, 2), (9000, 900)])
+def test_masked_logits(ctx, V, rows):
+    """-inf has no probability and comes last, lowest index first; a row of nothing else is defined."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(rows, V, generator=g)
+    x[0, torch.randperm(V, generator=g)[: V - 3]] = -math.inf
+    check(ctx, x, torch.zeros(rows, dtype=torch.int32), 5)
+    x[1] = -math.inf
+    lp, ent, tl, ti = (t.cpu() for t in ctx.token_logprobs(x.to(DEV), torch.zeros(rows, dtype=torch.int32, device=DEV), top=5))
+    assert lp[1] == -math.inf and ent[1] == 0 and (tl[1] == -math.inf).all() and ti[1].tolist() == [0, 1, 2, 3, 4]
+
+
+@pytest.mark.parametrize("V", [40, 9000, 70000])
+def test_nan_and_inf(ctx, V):
+    x = torch.randn(4, V, generator=torch.Generator().manual_seed(V))
+    x[0, 5] = math.nan
+    x[1, 7] = math.inf
+    x[2] = math.nan
+    x[2, 11], x[2, V - 1] = 1.0, -math.inf
+    lp, ent, tl, ti = (t.cpu() for t in ctx.token_logprobs(x.to(DEV), torch.zeros(4, dtype=torch.int32, device=DEV), top=4))
+    ctx.check()
+    assert torch.isnan(lp[:3]).all() and torch.isnan(ent[:3]).all() and torch.isnan(tl[:3]).all()
+    assert ti[1, 0] == 7 and ti[2].tolist() == [11, V - 1, 0, 1]
+    best = torch.sort(torch.nan_to_num(x[0], nan=-math.inf), descending=True, stable=True).indices[:4]
+    assert torch.equal(ti[0].long(), best)
+    check(ctx, x[3:], torch.tensor([3], dtype=torch.int32), 4)
+
+
+def test_tokens_none_and_out_of_range(ctx):
+    from q4k import Q4KError
+
+    x = torch.randn(3, 100)
+    lp, *_ = ctx.token_logprobs(x.to(DEV), torch.tensor([-1, 5, 99], dtype=torch.int32, device=DEV))
+    ctx.check()
+    assert torch.isnan(lp[0]) and torch.isfinite(lp[1:]).all()
+    lp, *_ = ctx.token_logprobs(x.to(DEV), torch.tensor([0, 100, 99], dtype=torch.int32, device=DEV))
+    with pytest.raises(Q4KError, match="token id"):
+        ctx.check()
+    assert torch.isnan(lp[1]) and torch.isfinite(lp[[0, 2]]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("offset,stride", [(0, 5003), (1, 5003), (3, 5001), (7, 5008)])
+def test_rows_at_any_alignment(ctx, dtype, offset, stride):
+    """Odd strides and starts; what lies between the rows is not read into them."""
+    V = 4990
+    buf = torch.full((6 * stride + 16,), 1e4, dtype=F32)
+    x = torch.randn(6, V, generator=torch.Generator().manual_seed(stride))
+    view = buf[offset : offset + 6 * stride].view(6, stride)
+    view[:, :V] = x
+    dev = buf.to(dtype).to(DEV)
+    rows = dev[offset : offset + 6 * stride].view(6, stride)[:, :V]
+    tokens = torch.arange(6, dtype=torch.int32)
+    lp, ent, tl, ti = (t.cpu() for t in ctx.token_logprobs(rows, tokens.to(DEV), top=6))
+    wl, we, wt, wi = reference(x.to(dtype), tokens, 6, 0.0)
+    assert ((lp - wl).abs() <= 1e-4).all() and ((ent - we).abs() <= 4e-4).all() and torch.equal(ti.long(), wi)
+
+
+def test_repeats_bit_for_bit_on_another_stream(ctx):
+    x = (torch.randn(3, 100001) * 3).to(DEV)
+    t = torch.zeros(3, dtype=torch.int32, device=DEV)
+    a = ctx.token_logprobs(x, t, top=20, cap=30.0)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        b = ctx.token_logprobs(x, t, top=20, cap=30.0)
+    torch.cuda.current_stream().wait_stream(s)
+    for u, v in zip(a, b):
+        assert torch.equal(u, v)
+
+
+def test_large_magnitudes(ctx):
+    x = torch.randn(2, 3000, generator=torch.Generator().manual_seed(1))
+    check(ctx, x * 1e4, torch.tensor([1, 2], dtype=torch.int32), 3)
+    check(ctx, x * 1e4, torch.tensor([1, 2], dtype=torch.int32), 3, cap=30.0)
+
+
+def test_refusals(ctx):
+    import q4k
+
+    x, t = torch.randn(2, 100, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV)
+    for args, err in [((x.double(), t), TypeError), ((x.cpu(), t), ValueError), ((x[0], t), ValueError),
+                      ((x.t(), t), ValueError), ((x, t.long()), TypeError), ((x, t[:1]), ValueError)]:
+        with pytest.raises(err):
+            ctx.token_logprobs(*args)
+    for top in (-1, 33, 101):
+        with pytest.raises(ValueError):
+            ctx.token_logprobs(x, t, top=top)
+    with pytest.raises(q4k.Q4KError):
+        ctx.token_logprobs(x, t, cap=float("nan"))
+    assert ctx.token_logprobs(x[:0], t[:0], top=3)[3].shape == (0, 3)
+    ctx.check()

@@ -1,0 +1,211 @@
+"""q4k_paged_attention on the GPU against the 64-bit restatement over the same
+codes.
+
+Bounds, relative to the output's 2-norm and to its largest value V.  f32 rows:
+scores carry 22 bits of the row and f32 sums over D terms, so a score of size
+|s| <= 30 (base 2: 44) is off by about 44 * 2^-21 = 2e-5 at worst and far less
+on average; 2-norm 2e-5, any element 2e-4 V.  f16 rows: 11 bits enter, so a
+score is off by up to 30 * 2^-11 at worst, on average by 1e-3: 2-norm 4e-3, any
+element 4e-2 V.  bf16 rows: their own rounding, 2^-9, besides: 2-norm 5e-3,
+any element 5e-2 V.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import kv_reference as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+NORM = {F32: 2e-5, F16: 4e-3, BF16: 5e-3}
+
+
+def close(got, want, dtype):
+    got, want = got.cpu().double(), want.double()
+    assert torch.isfinite(got).all()
+    norm = float(want.norm())
+    assert float((got - want).norm()) <= NORM[dtype] * max(norm, 1e-30)
+    assert float((got - want).abs().max()) <= 10 * NORM[dtype] * max(float(want.abs().max()), 1e-30)
+
+
+def run(ctx, pr, dtype, scale=None, window=0, **kw):
+    import q4k
+
+    cache, q, table, qs, kvl = pr.device(DEV, q4k, dtype)
+    scale = pr.d**-0.5 if scale is None else scale
+    out = ctx.paged_attention(cache, q, table, qs, kvl, max(pr.new), scale, window=window, **kw)
+    ctx.check()
+    return out
+
+
+HEADS = [(8, 1, 256), (8, 1, 512), (8, 2, 128), (3, 3, 64), (14, 2, 64), (20, 1, 128)]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("hq,hkv,d", HEADS)
+def test_decode_ragged(ctx, dtype, hq, hkv, d):
+    """Single tokens; lengths of one, around blocks and pages, empty ones."""
+    kv = [1, 15, 16, 17, 0, 33, 250, 64, 65, 700, 0, 129]
+    pr = R.Problem([1] * len(kv), kv, hq, hkv, d, 32, seed=d + hq)
+    close(run(ctx, pr, dtype), pr.expected(dtype, d**-0.5), dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("window", [0, 1, 20, 512])
+def test_few_tokens_windows_pages(ctx, dtype, page, window):
+    pr = R.Problem([3, 1, 4, 2, 0, 7], [3, 40, 700, 33, 20, 100], 8, 2, 128, page, seed=page + window)
+    close(run(ctx, pr, dtype, window=window), pr.expected(dtype, 128**-0.5, window), dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("hq,hkv,d,page,window", [(8, 1, 256, 16, 0), (8, 1, 256, 32, 100), (8, 1, 512, 64, 0),
+                                                  (8, 2, 128, 64, 0), (4, 4, 64, 128, 50), (12, 4, 128, 16, 0),
+                                                  (5, 1, 64, 32, 0)])
+def test_prompts(ctx, dtype, hq, hkv, d, page, window):
+    """Prompts of odd lengths, behind caches of odd lengths, beside single tokens and an empty sequence."""
+    new, past = [131, 1, 300, 0, 17, 64], [0, 75, 133, 10, 250, 64]
+    pr = R.Problem(new, [n + p for n, p in zip(new, past)], hq, hkv, d, page, seed=3 * d + hq)
+    close(run(ctx, pr, dtype, window=window), pr.expected(dtype, d**-0.5, window), dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_long_cache_is_split_and_merged(ctx, dtype):
+    """One row over a cache that many CTAs share (two levels of merging), and beside short ones."""
+    pr = R.Problem([1, 1, 2], [20000, 5, 3000], 8, 1, 256, 64, seed=2)
+    a = run(ctx, pr, dtype)
+    close(a, pr.expected(dtype, 256**-0.5), dtype)
+    for _ in range(3):
+        assert torch.equal(a, run(ctx, pr, dtype))  # the parts are added in their order
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("new", [1, 70])
+def test_value_blocks_of_any_magnitude(ctx, dtype, new):
+    pr = R.Problem([new], [400], 4, 1, 128, 16, seed=21, v_mix=True)
+    close(run(ctx, pr, dtype), pr.expected(dtype, 128**-0.5), dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("new", [1, 40])
+def test_peaked_flat_and_scaled_rows(ctx, dtype, new):
+    """Rows of zeros (flat weights), of large scores (one key decides) and of tiny and large magnitude."""
+    pr = R.Problem([new], [300], 4, 1, 64, 32, seed=23, spread=1.0)
+    pr.q[:, 0] = 0.0
+    pr.q[:, 1] *= 8.0
+    pr.q[:, 2] *= 1e-3
+    got, want = run(ctx, pr, dtype).cpu().double(), pr.expected(dtype, 64**-0.5)
+    for h in (0, 2, 3):
+        close(got[:, h], want[:, h], dtype)
+    # scores of up to 8 * 4 * 8: eight times the error of the others' scores
+    assert float((got[:, 1] - want[:, 1]).norm()) <= 8 * NORM[dtype] * float(want[:, 1].norm())
+
+
+@pytest.mark.parametrize("new", [1, 64])
+def test_what_is_masked_does_not_matter(ctx, new):
+    """Slots past the end may hold anything, NaN codes and scales among it;
+    rows of other sequences may be NaN."""
+    import q4k
+
+    pr = R.Problem([new, new], [new + 37, new + 20], 8, 2, 128, 64, seed=31)
+    want = pr.expected(BF16, 128**-0.5)
+    cache, q, table, qs, kvl = pr.device(DEV, q4k, BF16)
+    for b in range(2):
+        kv = pr.kv[b]
+        pg, slot = int(pr.table[b, (kv - 1) // 64]), (kv - 1) % 64 + 1
+        for c in (cache.k, cache.v):
+            c.view(torch.uint8)[pg, :, slot:] = 0x7F
+        for s in (cache.k_scale, cache.v_scale):
+            s[pg, :, (slot + 15) // 16 :] = float("nan")
+    q[new:] = float("nan")
+    got = ctx.paged_attention(cache, q, table, qs, kvl, new, 128**-0.5)
+    ctx.check()
+    close(got[:new], want[:new], BF16)
+    assert torch.isnan(got[new:]).all()
+
+
+@pytest.mark.parametrize("new", [1, 30])
+def test_no_position_no_weight(ctx, new):
+    """More new rows than tokens in the cache: the first rows have no position and are zero."""
+    pr = R.Problem([new], [max(0, new - 5)], 4, 1, 64, 16, seed=37)
+    got = run(ctx, pr, F32).cpu()
+    none = min(5, new)
+    assert (got[:none] == 0).all()
+    if new > 5:
+        sub = R.Problem([new - 5], [new - 5], 4, 1, 64, 16, seed=37)
+        sub.q, sub.k, sub.v, sub.k_scale, sub.v_scale, sub.table = pr.q[5:], pr.k, pr.v, pr.k_scale, pr.v_scale, pr.table
+        close(got[5:], sub.expected(F32, 64**-0.5), F32)
+
+
+def test_strides_streams_and_shared_pages(ctx):
+    """Rows out of a packed buffer, on another stream; two sequences that share their first pages."""
+    import q4k
+
+    pr = R.Problem([2, 3], [70, 75], 4, 2, 64, 16, seed=41)
+    pr.table[1, :3] = pr.table[0, :3]
+    want = pr.expected(BF16, 0.125)
+    cache, q, table, qs, kvl = pr.device(DEV, q4k, BF16)
+    buf = torch.zeros(5, 3, 256, dtype=BF16, device=DEV)
+    buf[:, 1] = q.flatten(1)
+    out = torch.full((5, 2, 256), 7.0, dtype=BF16, device=DEV)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    got = ctx.paged_attention(cache, buf[:, 1].view(5, 4, 64), table, qs, kvl, 3, 0.125, out=out[:, 0].view(5, 4, 64),
+                              stream=s)
+    torch.cuda.current_stream().wait_stream(s)
+    close(got, want, BF16)
+    assert (out[:, 1] == 7).all()
+
+
+def test_max_q_is_a_hint(ctx):
+    pr = R.Problem([50, 1], [80, 30], 8, 1, 128, 32, seed=43)
+    import q4k
+
+    want = pr.expected(F16, 128**-0.5)
+    cache, q, table, qs, kvl = pr.device(DEV, q4k, F16)
+    for hint in (0, 1, 49, 500):
+        close(ctx.paged_attention(cache, q, table, qs, kvl, hint, 128**-0.5), want, F16)
+
+
+@pytest.mark.parametrize("new", [1, 64])
+@pytest.mark.parametrize("what", ["page", "length", "rows"])
+def test_bad_metadata_is_reported(ctx, what, new):
+    import q4k
+
+    pr = R.Problem([new, new], [new + 9, new + 40], 8, 1, 128, 16, seed=47)
+    want = pr.expected(BF16, 128**-0.5)
+    cache, q, table, qs, kvl = pr.device(DEV, q4k, BF16)
+    if what == "page":
+        table[0, 0] = pr.pages + 1
+    elif what == "length":
+        kvl[0] = 1 << 20
+    else:
+        qs[2] = 2 * new + 100
+    got = ctx.paged_attention(cache, q, table, qs, kvl, new, 128**-0.5)
+    with pytest.raises(q4k.Q4KError, match="out of range"):
+        ctx.check()
+    if what == "rows":
+        close(got[:new], want[:new], BF16)
+    else:
+        close(got[new:], want[new:], BF16)
+
+
+def test_refusals(ctx):
+    import q4k
+
+    pr = R.Problem([2], [20], 4, 2, 64, 16)
+    cache, q, table, qs, kvl = pr.device(DEV, q4k, F32)
+    ok = dict(cache=cache, q=q, block_table=table, q_start=qs, kv_len=kvl, max_q=2, scale=0.125)
+    for change, err in [
+        (dict(q=q.double()), TypeError), (dict(q=q[:, :3]), q4k.Q4KError), (dict(q=q[:, :, :3]), ValueError),
+        (dict(q=q[:, :, :32]), ValueError), (dict(out=torch.empty_like(q).half()), TypeError),
+        (dict(window=-1), ValueError), (dict(max_q=-1), ValueError), (dict(scale=float("nan")), q4k.Q4KError),
+        (dict(kv_len=kvl.long()), TypeError), (dict(block_table=table.cpu()), ValueError),
+        (dict(q_start=qs[:1]), ValueError), (dict(q=q.cpu()), ValueError),
+    ]:
+        with pytest.raises(err):
+            ctx.paged_attention(**{**ok, **change})
+    assert ctx.paged_attention(**{**ok, "q": q[:0]}).shape == (0, 4, 64)
+    ctx.check()
