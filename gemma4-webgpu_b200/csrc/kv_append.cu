@@ -263,48 +263,50 @@ int kv_views(q4k_ctx* ctx, const char* what, const q4k_kv_cache* cache, const q4
 
 using namespace q4k;
 
-extern "C" int q4k_kv_append(q4k_ctx* ctx, const q4k_kv_cache* cache, const q4k_kv_batch* batch, uint32_t dtype,
-                             const void* k, uint64_t k_stride, const void* v, uint64_t v_stride, const float* rope,
-                             uint32_t rope_len, uint32_t rope_dim, const void* q, uint64_t q_stride, void* q_out,
-                             uint64_t q_out_stride, uint32_t q_heads, void* stream) {
+extern "C" int q4k_kv_append(q4k_ctx* ctx, const q4k_kv_cache* cache, const q4k_kv_batch* batch,
+                             const q4k_kv_append_args* args, void* stream) {
   if (!ctx) return Q4K_ERR_INVALID_ARG;
+  if (!args) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_kv_append: null arguments");
+  const q4k_kv_append_args& x = *args;
   AppendArgs a{};
-  const int rc = kv_views(ctx, "q4k_kv_append", cache, batch, dtype, q ? q_heads : 0, &a.c, &a.b);
+  const int rc = kv_views(ctx, "q4k_kv_append", cache, batch, x.dtype, x.q ? x.q_heads : 0, &a.c, &a.b);
   if (rc != Q4K_OK) return rc;
   if (a.b.tokens == 0 || a.b.seqs == 0) {
     ctx->err[0] = 0;
     return Q4K_OK;
   }
-  if (!k || !v || (q && (!q_out || q_heads == 0)))
+  if (!x.k || !x.v || (x.q && (!x.q_out || x.q_heads == 0)))
     return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_kv_append: null pointer");
   const uint32_t D = a.c.dim;
-  if (rope_dim % 16 != 0 || rope_dim > D || (rope_dim && (!rope || rope_len == 0)))
+  if (x.rope_dim % 16 != 0 || x.rope_dim > D || (x.rope_dim && (!x.rope || x.rope_len == 0)))
     return ctx_fail(ctx, Q4K_ERR_INVALID_ARG,
-                    "q4k_kv_append: rope_dim=%u must be a multiple of 16 up to head_dim=%u, with a table", rope_dim, D);
-  if (rope_dim && !aligned16(rope)) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_kv_append: rope must be 16-byte aligned");
-  const uint64_t kv_row = (uint64_t)a.c.heads * D, q_row = (uint64_t)q_heads * D;
-  if (!rows_ok(k, k_stride, kv_row, dtype) || !rows_ok(v, v_stride, kv_row, dtype) ||
-      (q && (!rows_ok(q, q_stride, q_row, dtype) || !rows_ok(q_out, q_out_stride, q_row, dtype))))
+                    "q4k_kv_append: rope_dim=%u must be a multiple of 16 up to head_dim=%u, with a table", x.rope_dim,
+                    D);
+  if (x.rope_dim && !aligned16(x.rope))
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_kv_append: rope must be 16-byte aligned");
+  const uint64_t kv_row = (uint64_t)a.c.heads * D, q_row = (uint64_t)x.q_heads * D;
+  if (!rows_ok(x.k, x.k_stride, kv_row, x.dtype) || !rows_ok(x.v, x.v_stride, kv_row, x.dtype) ||
+      (x.q && (!rows_ok(x.q, x.q_stride, q_row, x.dtype) || !rows_ok(x.q_out, x.q_out_stride, q_row, x.dtype))))
     return ctx_fail(ctx, Q4K_ERR_INVALID_ARG,
                     "q4k_kv_append: rows must be 16-byte aligned and at least heads * head_dim elements apart");
-  a.k = k;
-  a.v = v;
-  a.q = q;
-  a.q_out = q_out;
-  a.k_stride = k_stride;
-  a.v_stride = v_stride;
-  a.q_stride = q_stride;
-  a.qo_stride = q_out_stride;
-  a.q_heads = q ? q_heads : 0;
-  a.rope = rope;
-  a.rope_len = rope_len;
-  a.rot = rope_dim;
+  a.k = x.k;
+  a.v = x.v;
+  a.q = x.q;
+  a.q_out = x.q_out;
+  a.k_stride = x.k_stride;
+  a.v_stride = x.v_stride;
+  a.q_stride = x.q_stride;
+  a.qo_stride = x.q_out_stride;
+  a.q_heads = x.q ? x.q_heads : 0;
+  a.rope = x.rope;
+  a.rope_len = x.rope_len;
+  a.rot = x.rope_dim;
   a.status = ctx->select.status;
   const dim3 grid(a.b.tokens / 16 + 2 * a.b.seqs + 1, 2 * a.c.heads + (a.q_heads + kQHeadsPerCta - 1) / kQHeadsPerCta);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == Q4K_F32)
+  if (x.dtype == Q4K_F32)
     append_kernel<float><<<grid, D, 0, st>>>(a);
-  else if (dtype == Q4K_F16)
+  else if (x.dtype == Q4K_F16)
     append_kernel<__half><<<grid, D, 0, st>>>(a);
   else
     append_kernel<__nv_bfloat16><<<grid, D, 0, st>>>(a);

@@ -44,6 +44,7 @@ constexpr uint32_t kMergeGroup = 16;
 template <int D>
 struct AttendCfg {
   static constexpr int kWarps = D == 512 ? 4 : 8;
+  static constexpr int kCtas = 1;                        // CTAs an SM
   static constexpr int kStages = D >= 256 ? 3 : 4;
   static constexpr int kRow = D + 16;                    // bytes of a staged row: the pad spreads rows over the banks
   static constexpr int kStage = 2 * 16 * kRow + 16;      // 16 keys, 16 values, their scales
@@ -66,17 +67,18 @@ __device__ __forceinline__ void cp_wait() {
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
+
+__device__ __forceinline__ uint4 ld16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -93,6 +95,15 @@ __device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); 
 
 // 2^(m - top), 0 for an empty part.
 __device__ __forceinline__ float part_weight(float m, float top) { return m == neg_inf() ? 0.0f : ex2(m - top); }
+
+// Where a warp's result row keeps its 16-byte piece `u`: pieces are permuted
+// within groups of 8 so that the accumulators' stores (4 rows x 8 pieces 64
+// bytes apart) hit distinct banks, and so do loads of consecutive pieces.
+template <int D>
+__device__ __forceinline__ uint32_t piece(uint32_t row, uint32_t u) {
+  const uint32_t t = row >> 1 & 3u;
+  return (D >= 128 ? u ^ (t | (u >> 4 & 1u) << 2) : u ^ ((t & 1u) | (t >> 1) << 2)) * 4;
+}
 
 struct Seg {  // a sequence's share of the work
   KvSeq s;
@@ -113,7 +124,7 @@ __device__ __forceinline__ Seg seq_work(const AttendArgs& a, uint32_t b) {
 }
 
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, 1) attend_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas) attend_kernel(const AttendArgs a) {
   using C = AttendCfg<D>;
   constexpr bool kHiLo = Elem<T>::kExact;
   constexpr int R = 8 * NT;  // rows of a unit
@@ -123,42 +134,42 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, 1) attend_kernel(co
   uint8_t* const ring = smem;
   uint8_t* const qf = smem + C::kRing;  // [D / 16][NT][32 lanes] row operand in fragment order
   __shared__ float s_rs[R], s_m[C::kWarps][R], s_l[C::kWarps][R], s_f[2 * kMergeGroup][R], s_tot[R];
-  __shared__ unsigned long long s_scan[C::kWarps + 1];
-  __shared__ unsigned long long s_off;
-  __shared__ uint32_t s_seq, s_last;
+  __shared__ uint32_t s_scan[C::kWarps + 1];
+  __shared__ uint32_t s_off, s_seq, s_last;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
   const uint32_t H = a.c.heads, G = a.group;
-
-  // rows that see nothing, and sequences that cannot be served
-  for (uint32_t b = blockIdx.x; b < a.b.seqs; b += gridDim.x) {
-    const Seg w = seq_work<R>(a, b);
-    if (w.s.bad && tid == 0) atomicOr(a.status, kStatusKvMeta);
-    if (w.groups && w.blocks == 0) {
-      const uint32_t per = a.c.heads * G * D;
-      for (uint64_t i = tid; i < (uint64_t)w.s.n * per; i += kThreads)
-        static_cast<T*>(a.out)[(w.s.t0 + i / per) * a.out_stride + i % per] = Elem<T>::from(0.0f);
-    }
-  }
 
   // this CTA's range of the blocks of all units: each thread sums a run of
   // sequences, a scan over the threads finds the one the range starts in
   const uint32_t per_thread = (a.b.seqs + kThreads - 1) / kThreads;
   const uint32_t b_lo = min(tid * per_thread, a.b.seqs), b_hi = min(b_lo + per_thread, a.b.seqs);
-  unsigned long long mine = 0;
+  uint32_t mine = 0;
+  bool none = false;  // a sequence with rows that see nothing, or one that cannot be served
   for (uint32_t b = b_lo; b < b_hi; ++b) {
     const Seg w = seq_work<R>(a, b);
-    mine += (unsigned long long)w.blocks * w.groups * H;
+    mine += w.blocks * w.groups * H;  // 2^32 blocks would be 4 TB of the smallest cache
+    none |= w.s.bad || (w.groups && w.blocks == 0);
   }
-  unsigned long long scan = mine;
+  uint32_t scan = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long up = __shfl_up_sync(0xffffffffu, scan, o);
+    const uint32_t up = __shfl_up_sync(0xffffffffu, scan, o);
     if (lane >= (uint32_t)o) scan += up;
   }
   if (lane == 31) s_scan[warp + 1] = scan;
   if (tid == 0) s_scan[0] = 0;
-  __syncthreads();
-  unsigned long long total = 0, before = scan - mine;
+  if (__syncthreads_or(none)) {
+    for (uint32_t b = blockIdx.x; b < a.b.seqs; b += gridDim.x) {
+      const Seg w = seq_work<R>(a, b);
+      if (w.s.bad && tid == 0) atomicOr(a.status, kStatusKvMeta);
+      if (w.groups && w.blocks == 0) {
+        const uint32_t per = H * G * D;
+        for (uint64_t i = tid; i < (uint64_t)w.s.n * per; i += kThreads)
+          static_cast<T*>(a.out)[(w.s.t0 + i / per) * a.out_stride + i % per] = Elem<T>::from(0.0f);
+      }
+    }
+  }
+  uint32_t total = 0, before = scan - mine;
 #pragma unroll
   for (int i = 0; i < C::kWarps; ++i) {
     total += s_scan[i + 1];
@@ -166,16 +177,16 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, 1) attend_kernel(co
   }
   if (total == 0) return;
   // at least kWarps blocks a CTA: fewer leave warps idle and make more parts to merge
-  unsigned long long n_cta = (total + C::kWarps - 1) / C::kWarps;
-  n_cta = n_cta < gridDim.x ? n_cta : gridDim.x;
-  if (blockIdx.x >= n_cta) return;
-  unsigned long long cur = total * blockIdx.x / n_cta;
-  const unsigned long long end = total * (blockIdx.x + 1) / n_cta;
+  uint32_t quota = (total + gridDim.x - 1) / gridDim.x;
+  quota = quota < C::kWarps ? C::kWarps : quota;
+  uint32_t cur = quota * blockIdx.x;
+  if (cur >= total) return;
+  const uint32_t end = min(total, cur + quota);
   if (cur >= before && cur < before + mine) {
-    unsigned long long o = before;
+    uint32_t o = before;
     for (uint32_t b = b_lo; b < b_hi; ++b) {
       const Seg w = seq_work<R>(a, b);
-      const unsigned long long c = (unsigned long long)w.blocks * w.groups * H;
+      const uint32_t c = w.blocks * w.groups * H;
       if (cur < o + c) {
         s_seq = b;
         s_off = o;
@@ -186,22 +197,22 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, 1) attend_kernel(co
   }
   __syncthreads();
   uint32_t b = s_seq;
-  unsigned long long seq0 = s_off;  // global index of sequence b's first block
+  uint32_t seq0 = s_off;  // global index of sequence b's first block
 
   const uint32_t row_k = (g >> 1) + 4 * (g & 1);  // the key (of 8) that fragment row g holds: conflict-free with kRow
   const uint32_t ring_u = smem_u32(ring) + warp * C::kStages * C::kStage;
 
   while (cur < end) {
     const Seg w = seq_work<R>(a, b);
-    const unsigned long long cnt = (unsigned long long)w.blocks * w.groups * H;
+    const uint32_t cnt = w.blocks * w.groups * H;
     if (cur >= seq0 + cnt) {
       seq0 += cnt;
       ++b;
       continue;
     }
-    const uint32_t unit = (uint32_t)((cur - seq0) / w.blocks), u_off = (uint32_t)((cur - seq0) % w.blocks);
+    const uint32_t unit = (cur - seq0) / w.blocks, u_off = (cur - seq0) % w.blocks;
     const uint32_t h = unit / w.groups, rg = unit % w.groups;
-    const uint32_t n_blk = (uint32_t)min((unsigned long long)(w.blocks - u_off), end - cur);
+    const uint32_t n_blk = min(w.blocks - u_off, end - cur);
     const uint32_t blk0 = w.first + u_off;
     const uint32_t row0 = rg * R, n_rows = min((uint32_t)R, w.s.n * G - row0);
     const int pos0 = (int)w.s.kv - (int)w.s.n;
@@ -332,7 +343,7 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, 1) attend_kernel(co
       const uint8_t* kp = st + row_k * C::kRow + 16 * t;
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
-        const uint4 ka = lds128(kp + 64 * c), kb = lds128(kp + 8 * C::kRow + 64 * c);
+        const uint4 ka = ld16(kp + 64 * c), kb = ld16(kp + 8 * C::kRow + 64 * c);
         const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -342,7 +353,7 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, 1) attend_kernel(co
           for (int nt = 0; nt < NT; ++nt) {
             const uint8_t* q = qf + ((c * 4 + j) * NT + nt) * kQStep + lane * (kHiLo ? 16 : 8);
             if constexpr (kHiLo) {
-              const uint4 v = lds128(q);
+              const uint4 v = ld16(q);
               mma16816(s[0][nt], a0, a1, a2, a3, v.x, v.y);
               mma16816(s[1][nt], a0, a1, a2, a3, v.z, v.w);
             } else {
@@ -416,7 +427,7 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, 1) attend_kernel(co
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if constexpr (C::kVec == 16) {
-            const uint4 v = lds128(vp + 4 * k * C::kRow + 128 * ps);
+            const uint4 v = ld16(vp + 4 * k * C::kRow + 128 * ps);
             wv[k][0] = v.x, wv[k][1] = v.y, wv[k][2] = v.z, wv[k][3] = v.w;
           } else {
             const uint2 v = *reinterpret_cast<const uint2*>(vp + 4 * k * C::kRow);
@@ -463,7 +474,7 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, 1) attend_kernel(co
 #pragma unroll
         for (int k = 0; k < C::kPasses * (C::kVec / 4); ++k) {
           const uint32_t d = C::kVec == 16 ? 128 * (k / 4) + 16 * ((g >> 1) + 4 * (g & 1)) + 4 * (k % 4) : 8 * g + 4 * k;
-          *reinterpret_cast<float4*>(so + ((uint32_t)warp * R + r) * D + d) =
+          *reinterpret_cast<float4*>(so + ((uint32_t)warp * R + r) * D + piece<D>(r, d / 4)) =
               make_float4(o[k][0][nt][x], o[k][0][nt][2 + x], o[k][1][nt][x], o[k][1][nt][2 + x]);
         }
       }
@@ -482,8 +493,8 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, 1) attend_kernel(co
     __syncthreads();
 
     // a unit that lies within this CTA is written; a part of one goes to the workspace
-    const unsigned long long u0 = seq0 + (unsigned long long)unit * w.blocks, u1 = u0 + w.blocks;
-    const uint32_t c0 = (uint32_t)(((u0 + 1) * n_cta - 1) / total), c1 = (uint32_t)((u1 * n_cta - 1) / total);
+    const uint32_t u0 = seq0 + unit * w.blocks;
+    const uint32_t c0 = u0 / quota, c1 = (u0 + w.blocks - 1) / quota;
     const bool whole = c0 == c1;
     constexpr uint32_t kSlot = R * (D + 2);
     auto slot = [&](uint32_t i) {  // part i of this unit: CTA c0 keeps its last part apart from its first
@@ -501,7 +512,7 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, 1) attend_kernel(co
 #pragma unroll
       for (int k = 0; k < C::kWarps; ++k) {
         const float f = s_f[k][r];
-        const float4 y = *reinterpret_cast<const float4*>(so + ((uint32_t)k * R + r) * D + d);
+        const float4 y = *reinterpret_cast<const float4*>(so + ((uint32_t)k * R + r) * D + piece<D>(r, d / 4));
         v.x += y.x * f, v.y += y.y * f, v.z += y.z * f, v.w += y.w * f;
       }
       if (whole) {
@@ -548,11 +559,17 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, 1) attend_kernel(co
         for (uint32_t i = tid; i < n_rows * (D / 4); i += kThreads) {
           const uint32_t r = i / (D / 4), d = i % (D / 4) * 4;
           float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-          for (uint32_t k = 0; k < n; ++k) {
-            const float f = s_f[k][r];
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(slot(p0 + k * stride) + r * D + d));
-            v.x += y.x * f, v.y += y.y * f, v.z += y.z * f, v.w += y.w * f;
+          for (uint32_t k0 = 0; k0 < n; k0 += 8) {  // 8 loads in flight
+            float4 y[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k)
+              if (k0 + k < n) y[k] = __ldcg(reinterpret_cast<const float4*>(slot(p0 + (k0 + k) * stride) + r * D + d));
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k)
+              if (k0 + k < n) {
+                const float f = s_f[k0 + k][r];
+                v.x += y[k].x * f, v.y += y[k].y * f, v.z += y[k].z * f, v.w += y[k].w * f;
+              }
           }
           if (done) {
             const float tot = s_tot[r], inv = tot != 0.0f ? 1.0f / tot : 0.0f;
@@ -578,8 +595,13 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, 1) attend_kernel(co
 }
 
 template <int D, int NT, typename T>
-cudaError_t launch(const AttendArgs& a, uint32_t grid, int device, cudaStream_t s) {
+cudaError_t launch(const AttendArgs& a, uint32_t sms, int device, cudaStream_t s) {
   using C = AttendCfg<D>;
+  // two parts of every CTA fit the workspace
+  const size_t slot = 2 * 8 * NT * (D + 2) * sizeof(float);
+  uint32_t grid = sms * C::kCtas;
+  grid = grid < kAttendMaxCtas ? grid : kAttendMaxCtas;
+  grid = grid < a.work_bytes / slot ? grid : (uint32_t)(a.work_bytes / slot);
   constexpr int kSmem = C::kRing + (D / 16) * NT * 32 * (Elem<T>::kExact ? 16 : 8);
   static_assert(C::kWarps * 8 * NT * D * 4 <= C::kRing, "the warps' results fit the ring");
   static std::atomic<uint8_t> attr_set[kAttrDevices];
@@ -593,20 +615,20 @@ cudaError_t launch(const AttendArgs& a, uint32_t grid, int device, cudaStream_t 
 // then converted once for 16 rows.  At head dim 512 one group's accumulators
 // already take half the registers.
 template <int D, typename T>
-cudaError_t launch_rows(const AttendArgs& a, uint32_t rows, uint32_t grid, int device, cudaStream_t s) {
+cudaError_t launch_rows(const AttendArgs& a, uint32_t rows, uint32_t sms, int device, cudaStream_t s) {
   if constexpr (D < 512) {
-    if (rows > 8) return launch<D, 2, T>(a, grid, device, s);
+    if (rows > 8) return launch<D, 2, T>(a, sms, device, s);
   }
-  return launch<D, 1, T>(a, grid, device, s);
+  return launch<D, 1, T>(a, sms, device, s);
 }
 
 template <typename T>
-cudaError_t launch_dim(const AttendArgs& a, uint32_t rows, uint32_t grid, int device, cudaStream_t s) {
+cudaError_t launch_dim(const AttendArgs& a, uint32_t rows, uint32_t sms, int device, cudaStream_t s) {
   switch (a.c.dim) {
-    case 64: return launch_rows<64, T>(a, rows, grid, device, s);
-    case 128: return launch_rows<128, T>(a, rows, grid, device, s);
-    case 256: return launch_rows<256, T>(a, rows, grid, device, s);
-    default: return launch_rows<512, T>(a, rows, grid, device, s);
+    case 64: return launch_rows<64, T>(a, rows, sms, device, s);
+    case 128: return launch_rows<128, T>(a, rows, sms, device, s);
+    case 256: return launch_rows<256, T>(a, rows, sms, device, s);
+    default: return launch_rows<512, T>(a, rows, sms, device, s);
   }
 }
 
@@ -615,49 +637,47 @@ cudaError_t launch_dim(const AttendArgs& a, uint32_t rows, uint32_t grid, int de
 
 using namespace q4k;
 
-extern "C" int q4k_paged_attention(q4k_ctx* ctx, const q4k_kv_cache* cache, const q4k_kv_batch* batch, uint32_t dtype,
-                                   const void* q, uint64_t q_stride, void* out, uint64_t out_stride, uint32_t q_heads,
-                                   uint32_t max_q, float scale, uint32_t window, void* stream) {
+extern "C" int q4k_paged_attention(q4k_ctx* ctx, const q4k_kv_cache* cache, const q4k_kv_batch* batch,
+                                   const q4k_attention_args* args, void* stream) {
   if (!ctx) return Q4K_ERR_INVALID_ARG;
+  if (!args) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: null arguments");
+  const q4k_attention_args& x = *args;
   AttendArgs a{};
-  const int rc = kv_views(ctx, "q4k_paged_attention", cache, batch, dtype, q_heads, &a.c, &a.b);
+  const int rc = kv_views(ctx, "q4k_paged_attention", cache, batch, x.dtype, x.q_heads, &a.c, &a.b);
   if (rc != Q4K_OK) return rc;
   if (a.b.tokens == 0 || a.b.seqs == 0) {
     ctx->err[0] = 0;
     return Q4K_OK;
   }
-  if (!q || !out) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: null pointer");
-  if (q_heads == 0) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: q_heads must be >= 1");
-  if (!(scale == scale) || fabsf(scale) > 3.402823466e38f)
+  if (!x.q || !x.out) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: null pointer");
+  if (x.q_heads == 0) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: q_heads must be >= 1");
+  if (!(x.scale == x.scale) || fabsf(x.scale) > 3.402823466e38f)
     return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: scale must be finite");
-  if (window >= (1u << 31)) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: window=%u out of range", window);
-  const uint64_t row = (uint64_t)q_heads * a.c.dim;
-  if (!rows_ok(q, q_stride, row, dtype) || !rows_ok(out, out_stride, row, dtype))
+  if (x.window >= (1u << 31)) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: window=%u out of range", x.window);
+  const uint64_t row = (uint64_t)x.q_heads * a.c.dim;
+  if (!rows_ok(x.q, x.q_stride, row, x.dtype) || !rows_ok(x.out, x.out_stride, row, x.dtype))
     return ctx_fail(ctx, Q4K_ERR_INVALID_ARG,
                     "q4k_paged_attention: rows must be 16-byte aligned and at least q_heads * head_dim elements apart");
-  a.q = q;
-  a.out = out;
-  a.q_stride = q_stride;
-  a.out_stride = out_stride;
-  a.group = q_heads / a.c.heads;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.window = window;
+  a.q = x.q;
+  a.out = x.out;
+  a.q_stride = x.q_stride;
+  a.out_stride = x.out_stride;
+  a.group = x.q_heads / a.c.heads;
+  a.scale_log2 = x.scale * 1.4426950408889634f;
+  a.window = x.window;
   a.work = reinterpret_cast<float*>(ctx->xfrag);
+  a.work_bytes = ctx->xfrag_cap;
   a.counters = ctx->split_counters;
   a.status = ctx->select.status;
   // prompts go to the tile kernel, sequence by sequence; f32 rows keep to this one, whose f32 accuracy it lacks
-  uint32_t rows = max_q > (1u << 24) ? 1u << 30 : (max_q ? max_q : 1) * a.group;
-  const bool prompts = dtype != Q4K_F32 && rows > kPromptRows;
+  uint32_t rows = x.max_q > (1u << 24) ? 1u << 30 : (x.max_q ? x.max_q : 1) * a.group;
+  const bool prompts = x.dtype != Q4K_F32 && rows > kPromptRows;
   a.max_rows = prompts ? kPromptRows : 0;
   const bool all = prompts && a.b.seqs == 1 && a.b.tokens * a.group > kPromptRows;  // no other sequence is left
-  const uint32_t grid = (uint32_t)ctx->sm_count;
-  static_assert(2 * 160 * 16 * (256 + 2) * 4 <= kCtxXfragBytes, "two parts a CTA fit the context's scratch");
-  if (grid > kAttendMaxCtas || (size_t)2 * grid * (a.c.dim == 512 ? 8 : 16) * (a.c.dim + 2) * 4 > ctx->xfrag_cap)
-    return ctx_fail(ctx, Q4K_ERR_UNSUPPORTED, "q4k_paged_attention: %u SMs need more scratch than the context has", grid);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
   if (prompts) {
-    e = launch_prompt(a, dtype, ctx->select.spin_limit, ctx->device, st);
+    e = launch_prompt(a, x.dtype, ctx->select.spin_limit, ctx->device, st);
     if (e != cudaSuccess) return ctx_cuda(ctx, e, "q4k_paged_attention prompt launch");
     rows = kPromptRows;
   }
@@ -665,11 +685,11 @@ extern "C" int q4k_paged_attention(q4k_ctx* ctx, const q4k_kv_cache* cache, cons
     ctx->err[0] = 0;
     return Q4K_OK;
   }
-  if (dtype == Q4K_F32)
-    e = launch_dim<float>(a, rows, grid, ctx->device, st);
-  else if (dtype == Q4K_F16)
-    e = launch_dim<__half>(a, rows, grid, ctx->device, st);
+  if (x.dtype == Q4K_F32)
+    e = launch_dim<float>(a, rows, (uint32_t)ctx->sm_count, ctx->device, st);
+  else if (x.dtype == Q4K_F16)
+    e = launch_dim<__half>(a, rows, (uint32_t)ctx->sm_count, ctx->device, st);
   else
-    e = launch_dim<__nv_bfloat16>(a, rows, grid, ctx->device, st);
+    e = launch_dim<__nv_bfloat16>(a, rows, (uint32_t)ctx->sm_count, ctx->device, st);
   return ctx_cuda(ctx, e, "q4k_paged_attention launch");
 }

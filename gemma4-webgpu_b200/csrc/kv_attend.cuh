@@ -20,6 +20,7 @@ struct AttendArgs {
   uint32_t max_rows;  // sequences with more rows a key head are another kernel's (0: none are)
   float scale_log2;   // softmax scale * log2(e)
   float* work;        // parts of cut units: 2 per CTA
+  size_t work_bytes;
   uint32_t* counters;
   uint32_t* status;
 };

@@ -8,16 +8,17 @@
 //   lse = ln 2 (m + log2 s),  entropy = ln 2 (log2 s - w / s).
 // The softcap is monotone, so alternatives are chosen by the raw logits.
 //
-// A CTA takes a row, or a part of one when there are few rows, in tiles held
-// in registers.  Each thread keeps its own (m, s, w).  Alternatives: the
-// k-th largest of the threads' tile maxima bounds the k-th largest logit from
-// below, so after the first tile only a few more than k elements pass the
-// bound; they go to a list in shared memory that is cut back to k (by each
-// entry's rank) when it has grown, which raises the bound.  A tile whose
-// passing elements overflow the list (many equal logits) is searched k times
-// instead.  The order is a 64-bit key, value then inverted index, so ties go
-// to the lowest index and no two keys are equal: the result does not depend
-// on the order of arrival.
+// A CTA takes a part of a row, at most kLpTiles tiles of 16 KB, and streams it
+// without a barrier: each thread keeps its own (m, s, w) and the largest
+// element of each of its tiles.  Alternatives: the k-th largest of the
+// threads' maxima bounds the part's k-th largest logit from below, so little
+// more than k elements pass it, and they lie in the few (thread, tile) pairs
+// whose maximum passes; those are read again (from L2), a warp a pair, and the
+// elements that pass are ranked in shared memory.  A part whose pairs or
+// elements overflow their list (many equal logits) is searched k times instead.  The order is a 64-bit key, value
+// then inverted index, so ties go to the lowest index and no two keys are
+// equal: the result does not depend on the order of arrival.  The part that
+// finishes last merges a row's parts in their order.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -31,20 +32,24 @@ constexpr uint32_t kLpThreads = 256;
 constexpr uint32_t kLpVecs = 4;      // 16-byte loads a thread and tile
 constexpr uint32_t kLpTop = 32;      // most alternatives
 constexpr uint32_t kLpList = 1024;   // list entries (kLpTop - 1 parts of kLpTop keys fit)
-constexpr uint32_t kLpPrune = 64;    // entries at which the list is cut back
+constexpr uint32_t kLpTiles = 16;    // most tiles of a part
+constexpr uint32_t kLpHits = 512;    // most (thread, tile) pairs that are read again
+constexpr uint32_t kLpParts = 64;    // most parts of a row
+constexpr uint32_t kLpRounds = 1;    // rounds of CTAs that a launch should have before its parts grow
+constexpr uint32_t kLpMaxV = kLpParts * kLpTiles * kLpThreads * kLpVecs * 4;  // f32 elements of the most tiles
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct LpPart {  // what a part of a row leaves for the merge
-  float m, s, w;
-  uint32_t n;
+  float m, s, w, unused;
   unsigned long long key[kLpTop];
 };
 
 struct LpArgs {
   const void* logits;
   uint64_t stride;
-  uint32_t rows, V, splits, top;
-  float cap;
+  uint32_t row0, V, splits, top;  // row0: first row of this launch
+  uint32_t part_vecs;             // 16-byte vectors of a part, a multiple of kLpThreads
+  float cap, cap_rate;  // 0: none; 2 log2(e) / cap
   const int32_t* tokens;
   float* logprob;
   float* entropy;
@@ -81,35 +86,82 @@ __device__ __forceinline__ unsigned long long key_of(float x, uint32_t idx) {
   return ((unsigned long long)ord_of(x) << 32) | (0xffffffffu - idx);
 }
 
-// cap tanh(x / cap) = cap - 2 cap / (2^(2 log2(e) x / cap) + 1).
-__device__ __forceinline__ float capped(float x, float cap) {
-  if (cap <= 0.0f) return x;
-  return cap - __fdividef(2.0f * cap, lp_ex2(x * (2.0f * kLog2e / cap)) + 1.0f);
+// A logit's softcapped value: cap tanh(v / cap) = cap - 2 cap / (2^(2 log2(e) v / cap) + 1).
+template <bool kCap>
+__device__ __forceinline__ float capped(float v, const LpArgs& a) {
+  if (!kCap) return v;
+  return fmaf(-2.0f * a.cap, __fdividef(1.0f, lp_ex2(v * a.cap_rate) + 1.0f), a.cap);
+}
+
+// The elements of a 16-byte vector.
+__device__ __forceinline__ void unpack(const uint4& w, float (&e)[4], const float*) {
+  e[0] = __uint_as_float(w.x), e[1] = __uint_as_float(w.y), e[2] = __uint_as_float(w.z), e[3] = __uint_as_float(w.w);
+}
+__device__ __forceinline__ void unpack(const uint4& w, float (&e)[8], const __nv_bfloat16*) {
+  const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    e[2 * i] = __uint_as_float(p[i] << 16);
+    e[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack(const uint4& w, float (&e)[8], const __half*) {
+  const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[i]));
+    e[2 * i] = f.x;
+    e[2 * i + 1] = f.y;
+  }
+}
+
+// Two f32 operations an instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return r;
 }
 
 struct Stats {
-  float m, s, w;  // m = -inf: nothing yet
+  float m, s, w;  // m: the reference in the logits' units, -inf: nothing yet
 };
+// 2^((x - m) log2 e) and its exponent, for any x and m (m = -inf: nothing above -inf yet): -inf adds nothing.
+__device__ __forceinline__ float below(float x, float m) {
+  return max_nan((x - (m == neg_inf() ? 0.0f : m)) * kLog2e, -252.0f);  // 2^-252 is 0
+}
 __device__ __forceinline__ void rebase(Stats& a, float m) {  // to a larger reference
   if (a.m == m) return;
   if (a.m != neg_inf()) {
-    const float d = a.m - m, f = lp_ex2(d);
-    // a.s == 0: nothing but -inf so far
-    a.w = f * (a.w + a.s * max_nan(d, -252.0f));
+    const float d = below(a.m, m), f = lp_ex2(d);
+    a.w = f * fmaf(a.s, d, a.w);
     a.s *= f;
   }
   a.m = m;
 }
-__device__ __forceinline__ Stats merge(Stats a, Stats b) {
-  const float m = fmaxf(a.m, b.m);
-  rebase(a, m);
-  rebase(b, m);
-  return Stats{m, a.s + b.s, a.w + b.w};
+// The sum of every lane's statistics under their common largest reference.
+__device__ __forceinline__ float warp_max(float m) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+__device__ __forceinline__ Stats warp_merge(Stats st, float m) {
+  rebase(st, m);
+  return Stats{m, warp_sum(st.s), warp_sum(st.w)};
 }
 
-// The list's entries by rank: the `k` largest first, in order.  All threads.
-__device__ __forceinline__ uint32_t prune(unsigned long long* list, uint32_t n, uint32_t k) {
-  __syncthreads();
+// The k largest of the list's n entries (no two equal) to its front, in
+// order, by each entry's rank.  All threads; returns how many there are.
+__device__ __forceinline__ uint32_t rank_list(unsigned long long* list, uint32_t n, uint32_t k) {
   unsigned long long mine[kLpList / kLpThreads];
   uint32_t rank[kLpList / kLpThreads];
 #pragma unroll
@@ -118,6 +170,7 @@ __device__ __forceinline__ uint32_t prune(unsigned long long* list, uint32_t n, 
     mine[i] = at < n ? list[at] : 0ull;
     rank[i] = 0;
     if (at < n)
+#pragma unroll 8
       for (uint32_t j = 0; j < n; ++j) rank[i] += list[j] > mine[i];
   }
   __syncthreads();
@@ -128,225 +181,292 @@ __device__ __forceinline__ uint32_t prune(unsigned long long* list, uint32_t n, 
   return min(n, k);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
+template <typename T, bool kCap>
+__global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a) {
   constexpr uint32_t kVE = 16 / sizeof(T);  // elements of a vector
-  constexpr uint32_t kN = kLpVecs * kVE;    // elements a thread and tile
+  constexpr uint32_t kWarps = kLpThreads / 32;
+  const T* const kTag = nullptr;
   __shared__ unsigned long long s_list[kLpList];
-  __shared__ unsigned long long s_key[kLpThreads / 32];
-  __shared__ Stats s_stats[kLpThreads / 32];
-  __shared__ uint32_t s_n, s_last;
+  __shared__ unsigned long long s_key[kWarps];
+  __shared__ Stats s_stats[kWarps];
+  __shared__ float s_top[kWarps], s_tile[kLpTiles][kLpThreads];  // warps' references; threads' tile maxima
+  __shared__ uint32_t s_max[kLpThreads];
+  __shared__ uint16_t s_hit[kLpHits];  // tile * kLpThreads + thread
+  __shared__ uint32_t s_n, s_hits, s_last, s_bound;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-  const uint32_t row = blockIdx.x / a.splits, part = blockIdx.x % a.splits;
+  const uint32_t lrow = blockIdx.x / a.splits, row = a.row0 + lrow, part = blockIdx.x % a.splits;
   const T* const x = static_cast<const T*>(a.logits) + (uint64_t)row * a.stride;
-  // vectors of 16 aligned bytes; the first and last may hold elements of no row
+  // the row's whole 16-byte vectors, and `head` elements before and some after them
   const uint32_t mis = (uint32_t)(((uintptr_t)x & 15u) / sizeof(T));
-  const uint32_t n_vec = (a.V + mis + kVE - 1) / kVE, per = (n_vec + a.splits - 1) / a.splits;
-  const uint32_t v_lo = min(part * per, n_vec), v_hi = min(v_lo + per, n_vec);
+  const uint32_t head = min(mis ? kVE - mis : 0u, a.V), n_vec = (a.V - head) / kVE, tail0 = head + n_vec * kVE;
+  const T* const xv = x + head;
+  const uint32_t v_lo = min(part * a.part_vecs, n_vec), v_hi = min(v_lo + a.part_vecs, n_vec);
   const uint32_t k = a.top;
+  // a ragged element of this thread's: the head's in the first part, the tail's in the last
+  uint32_t odd = 0xffffffffu;
+  if (part == 0 && tid < head) odd = tid;
+  if (part == a.splits - 1 && tid >= 16 && tail0 + (tid - 16) < a.V) odd = tail0 + (tid - 16);
 
   Stats st{neg_inf(), 0.0f, 0.0f};
-  uint32_t n_list = 0;      // entries of the list (the same in every thread)
-  float bound = neg_inf();  // an element enters the list if above it
-  bool first = true, equal = true;  // equal: also one equal to the bound
-  if (tid == 0) s_n = 0;
-  __syncthreads();
+  float best = neg_inf();  // the thread's largest element
+  bool any = odd != 0xffffffffu;
+  if (any) {
+    best = Elem<T>::to(x[odd]);
+    const float c = capped<kCap>(best, a);
+    st.m = fmaxf(c, neg_inf());  // NaN does not become the reference
+    const float d = below(c, st.m);
+    st.s = lp_ex2(d);
+    st.w = st.s * d;
+  }
 
-  for (uint32_t v0 = v_lo; v0 < v_hi; v0 += kLpThreads * kLpVecs, first = false) {
-    float e[kN];
-    uint32_t ok = 0;  // bit i: element i is one of the row's
-    uint4 raw[kLpVecs];
+  uint4 raw[kLpVecs];
+#pragma unroll
+  for (uint32_t i = 0; i < kLpVecs; ++i)
+    if (v_lo + i * kLpThreads + tid < v_hi) raw[i] = ldg_nc_v4(xv + (uint64_t)(v_lo + i * kLpThreads + tid) * kVE);
+#pragma unroll 1
+  for (uint32_t t = 0; t * kLpThreads * kLpVecs < a.part_vecs; ++t) {
+    const uint32_t v0 = v_lo + t * kLpThreads * kLpVecs + tid;
+    if (v0 >= v_hi) break;
+    uint4 cur[kLpVecs];
+#pragma unroll
+    for (uint32_t i = 0; i < kLpVecs; ++i) cur[i] = raw[i];
+#pragma unroll
+    for (uint32_t i = 0; i < kLpVecs; ++i) {  // the next tile is on its way while this one is reduced
+      const uint32_t v = v0 + (kLpVecs + i) * kLpThreads;
+      if (v < v_hi) raw[i] = ldg_nc_v4(xv + (uint64_t)v * kVE);
+    }
+    float mx = __int_as_float(0x7fc00000);
 #pragma unroll
     for (uint32_t i = 0; i < kLpVecs; ++i) {
-      const uint32_t v = v0 + i * kLpThreads + tid;
-      const bool in = v < v_hi && v * kVE >= mis && (v + 1) * kVE - mis <= a.V;
-      if (in) {
-        raw[i] = ldg_nc_v4(x + (int64_t)(v * kVE) - mis);
-        ok |= ((1u << kVE) - 1u) << (i * kVE);
+      if (v0 + i * kLpThreads < v_hi) {
+        float e[kVE];
+        unpack(cur[i], e, kTag);
+#pragma unroll
+        for (uint32_t j = 0; j < kVE; ++j) mx = fmaxf(mx, e[j]);
       }
     }
+    any = true;
+    s_tile[t][tid] = mx;
+    best = fmaxf(best, mx);
+    const float top = capped<kCap>(mx, a);
+    if (top > st.m) rebase(st, top);
+    const float ref = -st.m * kLog2e;
+    float2 ss = make_float2(0.0f, 0.0f), ws = ss;
+    const float2 ref2 = make_float2(ref, ref), rate2 = make_float2(kLog2e, kLog2e);
 #pragma unroll
     for (uint32_t i = 0; i < kLpVecs; ++i) {
-      const uint32_t v = v0 + i * kLpThreads + tid;
-      if (ok >> (i * kVE) & 1u) {
-        const T* p = reinterpret_cast<const T*>(&raw[i]);
+      if (v0 + i * kLpThreads < v_hi) {
+        float e[kVE];
+        unpack(cur[i], e, kTag);
 #pragma unroll
-        for (uint32_t j = 0; j < kVE; ++j) e[i * kVE + j] = Elem<T>::to(p[j]);
-      } else {
+        for (uint32_t j = 0; j < kVE; j += 2) {
+          const float2 d = fma2(make_float2(capped<kCap>(e[j], a), capped<kCap>(e[j + 1], a)), rate2, ref2);
+          const float2 p = make_float2(lp_ex2(d.x), lp_ex2(d.y));
+          ss = add2(ss, p);
+          ws = fma2(p, d, ws);
+        }
+      }
+    }
+    float s0 = ss.x + ss.y, w0 = ws.x + ws.y;
+    if (!(fabsf(w0) <= 3.402823466e38f)) {  // -inf, NaN, or values near the end of f32's range: term by term
+      s0 = w0 = 0.0f;
+#pragma unroll 1
+      for (uint32_t i = 0; i < kLpVecs; ++i) {
+        if (v0 + i * kLpThreads < v_hi) {
+          float e[kVE];
+          unpack(ldg_nc_v4(xv + (uint64_t)(v0 + i * kLpThreads) * kVE), e, kTag);
 #pragma unroll
-        for (uint32_t j = 0; j < kVE; ++j) {
-          const int64_t at = (int64_t)(v * kVE + j) - mis;
-          e[i * kVE + j] = neg_inf();
-          if (v < v_hi && at >= 0 && at < (int64_t)a.V) {
-            e[i * kVE + j] = Elem<T>::to(x[at]);
-            ok |= 1u << (i * kVE + j);
+          for (uint32_t j = 0; j < kVE; ++j) {
+            const float d = below(capped<kCap>(e[j], a), st.m), p = lp_ex2(d);
+            s0 += p;
+            w0 = fmaf(p, d, w0);
           }
         }
       }
     }
-    float mx = e[0];
-#pragma unroll
-    for (uint32_t j = 1; j < kN; ++j) mx = fmaxf(mx, e[j]);
-
-    // statistics
-    {
-      const float top = capped(mx, a.cap) * kLog2e;
-      if (top > st.m) rebase(st, top);
-      const float ref = st.m == neg_inf() ? 0.0f : st.m;
-#pragma unroll
-      for (uint32_t j = 0; j < kN; ++j) {
-        const float d = max_nan(fmaf(capped(e[j], a.cap), kLog2e, -ref), -252.0f);  // 2^-252 is 0: -inf adds nothing
-        const float p = lp_ex2(d);
-        st.s += p;
-        st.w = fmaf(p, d, st.w);
-      }
-    }
-    if (k == 0) continue;
-
-    // alternatives
-    if (first) {
-      const uint32_t mine = ok ? ord_of(mx) : 0u;
-      uint32_t t = 0;  // the largest prefix that k threads' maxima reach
-      for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
-        if (__syncthreads_count(mine >= (t | bit)) >= (int)k) t |= bit;
-      bound = t ? of_ord(t) : neg_inf();
-      if (!(bound == bound)) bound = neg_inf();  // a prefix within NaN's codes
-    }
-    const bool mine = equal ? mx >= bound : mx > bound;
-    if (mine) {
-#pragma unroll
-      for (uint32_t j = 0; j < kN; ++j) {
-        if ((equal ? e[j] >= bound : e[j] > bound) && (ok >> j & 1u)) {
-          const uint32_t at = atomicAdd(&s_n, 1u);
-          const uint32_t v = v0 + (j / kVE) * kLpThreads + tid;
-          if (at < kLpList) s_list[at] = key_of(e[j], v * kVE + j % kVE - mis);
-        }
-      }
-    }
-    if (!__syncthreads_or(mine) && !first) continue;
-    uint32_t n = s_n;
-    // the first tile owes k entries (or all that it has, were they NaN)
-    const bool owe = first && n < k;
-    if (n > kLpList || owe) {
-      // search the tile itself: the largest key below the last, k times
-      unsigned long long below = ~0ull;
-      n = n_list;
-      for (uint32_t r = 0; r < k; ++r) {
-        unsigned long long best = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < kN; ++j) {
-          const uint32_t v = v0 + (j / kVE) * kLpThreads + tid;
-          const unsigned long long key = key_of(e[j], v * kVE + j % kVE - mis);
-          if ((ok >> j & 1u) && key < below && key > best) best = key;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-          best = other > best ? other : best;
-        }
-        __syncthreads();
-        if (lane == 0) s_key[warp] = best;
-        __syncthreads();
-#pragma unroll
-        for (uint32_t i = 0; i < kLpThreads / 32; ++i) best = s_key[i] > best ? s_key[i] : best;
-        if (best == 0) break;
-        if (tid == 0) s_list[n] = best;
-        ++n;
-        below = best;
-      }
-    }
-    if (first || n > kLpPrune) {
-      n = prune(s_list, n, k);
-      // later elements have higher indices: one equal to the k-th loses
-      if (n == k) bound = of_ord((uint32_t)(s_list[k - 1] >> 32));
-      equal = n < k || !(bound == bound);  // a NaN among the k yields to any number
-      if (equal) bound = neg_inf();
-    }
-    n_list = n;
-    __syncthreads();
-    if (tid == 0) s_n = n;
-    __syncthreads();
+    st.s += s0;
+    st.w += w0;
   }
-  if (k && n_list > 0) n_list = prune(s_list, n_list, k);
 
-  // the CTA's statistics, in thread 0's order of warps
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stats other;
-    other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-    other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    other.w = __shfl_xor_sync(0xffffffffu, st.w, o);
-    st = merge(st, other);
+  // the CTA's statistics under its largest reference, the warps' sums in their
+  // order; meanwhile warp 0 finds the bound: the largest 16-bit prefix of the
+  // order that k threads' maxima reach
+  s_max[tid] = any ? ord_of(best) : 0u;
+  {
+    const float top = warp_max(st.m);
+    if (lane == 0) s_top[warp] = top;
   }
-  if (lane == 0) s_stats[warp] = st;
+  if (tid == 0) s_n = s_hits = 0;
+  __syncthreads();
+  if (warp == 0 && k) {
+    uint32_t o[kWarps];
+#pragma unroll
+    for (uint32_t i = 0; i < kWarps; ++i) o[i] = s_max[i * 32 + lane] >> 16;
+    uint32_t t = 0;
+    for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+      uint32_t c = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < kWarps; ++i) c += o[i] >= (t | bit);
+      if (__reduce_add_sync(0xffffffffu, c) >= k) t |= bit;
+    }
+    if (lane == 0) s_bound = t << 16;
+  }
+  {
+    float m = s_top[0];
+#pragma unroll
+    for (uint32_t i = 1; i < kWarps; ++i) m = fmaxf(m, s_top[i]);
+    st = warp_merge(st, m);
+    if (lane == 0) s_stats[warp] = st;
+  }
   __syncthreads();
   st = s_stats[0];
 #pragma unroll
-  for (uint32_t i = 1; i < kLpThreads / 32; ++i) st = merge(st, s_stats[i]);
+  for (uint32_t i = 1; i < kWarps; ++i) st.s += s_stats[i].s, st.w += s_stats[i].w;
+
+  uint32_t n_list = 0;
+  if (k) {
+    float bound = s_bound ? of_ord(s_bound) : neg_inf();
+    if (!(bound == bound)) bound = neg_inf();  // a prefix within NaN's codes
+    auto push = [&](float e, uint32_t idx) {
+      if (e >= bound) {
+        const uint32_t at = atomicAdd(&s_n, 1u);
+        if (at < kLpList) s_list[at] = key_of(e, idx);
+      }
+    };
+    if (best >= bound) {
+      if (odd != 0xffffffffu) push(Elem<T>::to(x[odd]), odd);
+#pragma unroll 1
+      for (uint32_t t = 0; v_lo + t * kLpThreads * kLpVecs + tid < v_hi; ++t) {
+        if (s_tile[t][tid] >= bound) {
+          const uint32_t at = atomicAdd(&s_hits, 1u);
+          if (at < kLpHits) s_hit[at] = (uint16_t)(t * kLpThreads + tid);
+        }
+      }
+    }
+    __syncthreads();
+    const uint32_t hits = s_hits;
+    if (hits <= kLpHits) {
+      // a pair's kLpVecs vectors hold kLpVecs * kVE <= 32 elements, one a lane
+#pragma unroll 2
+      for (uint32_t i = warp; i < hits; i += kWarps) {
+        const uint32_t t = s_hit[i] / kLpThreads, th = s_hit[i] % kLpThreads;
+        const uint32_t v = v_lo + t * kLpThreads * kLpVecs + th + (lane / kVE) * kLpThreads;
+        if (lane < kLpVecs * kVE && v < v_hi) push(Elem<T>::to(xv[(uint64_t)v * kVE + lane % kVE]), head + v * kVE + lane % kVE);
+      }
+    }
+    __syncthreads();
+    n_list = hits <= kLpHits ? s_n : kLpList + 1;
+    const uint64_t have = (uint64_t)(v_hi - v_lo) * kVE + (part == 0 ? head : 0) +
+                          (part == a.splits - 1 ? a.V - tail0 : 0);  // elements of the part
+    if (n_list > kLpList || n_list < (have < k ? (uint32_t)have : k)) {
+      // too many equal ones, or NaN among the k largest: the largest key below the last, k times
+      unsigned long long last = ~0ull;
+      n_list = 0;
+      for (uint32_t r = 0; r < k; ++r) {
+        unsigned long long top = 0;
+        auto take = [&](float e, uint32_t idx) {
+          const unsigned long long key = key_of(e, idx);
+          if (key < last && key > top) top = key;
+        };
+        if (odd != 0xffffffffu) take(Elem<T>::to(x[odd]), odd);
+        for (uint32_t v = v_lo + tid; v < v_hi; v += kLpThreads) {
+          float e[kVE];
+          unpack(ldg_nc_v4(xv + (uint64_t)v * kVE), e, kTag);
+          for (uint32_t j = 0; j < kVE; ++j) take(e[j], head + v * kVE + j);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const unsigned long long other = __shfl_xor_sync(0xffffffffu, top, o);
+          top = other > top ? other : top;
+        }
+        __syncthreads();
+        if (lane == 0) s_key[warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < kWarps; ++i) top = s_key[i] > top ? s_key[i] : top;
+        if (top == 0) break;
+        if (tid == 0) s_list[n_list] = top;
+        ++n_list;
+        last = top;
+      }
+      __syncthreads();
+    } else {
+      n_list = rank_list(s_list, n_list, k);
+    }
+  }
 
   if (a.splits > 1) {
-    LpPart* const ps = a.parts + (uint64_t)row * a.splits;
+    LpPart* const ps = a.parts + (uint64_t)lrow * a.splits;
     if (tid == 0) {
       ps[part].m = st.m;
       ps[part].s = st.s;
       ps[part].w = st.w;
-      ps[part].n = n_list;
     }
     if (tid < k) ps[part].key[tid] = tid < n_list ? s_list[tid] : 0ull;
     __syncthreads();
     if (tid == 0) {
       __threadfence();
-      s_last = atomicAdd(&a.counters[row], 1u) == a.splits - 1;
-      if (s_last) a.counters[row] = 0;
+      s_last = atomicAdd(&a.counters[lrow], 1u) == a.splits - 1;
+      if (s_last) a.counters[lrow] = 0;
       s_n = 0;
     }
     __syncthreads();
     if (!s_last) return;
     __threadfence();
-    // parts in their order: thread i holds part i's statistics and largest key
-    st = Stats{neg_inf(), 0.0f, 0.0f};
-    for (uint32_t i = lane; i < a.splits; i += 32)
-      st = merge(st, Stats{__ldcg(&ps[i].m), __ldcg(&ps[i].s), __ldcg(&ps[i].w)});
+    // every warp merges the parts' statistics, in the same order
+    const unsigned long long head_key = k && tid < a.splits ? __ldcg(&ps[tid].key[0]) : 0ull;
+    Stats two[kLpParts / 32];
+    float m = neg_inf();
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      Stats other;
-      other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-      other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-      other.w = __shfl_xor_sync(0xffffffffu, st.w, o);
-      st = merge(st, other);
+    for (uint32_t i = 0; i < kLpParts / 32; ++i) {
+      two[i] = Stats{neg_inf(), 0.0f, 0.0f};
+      if (lane + 32 * i < a.splits) {
+        const float4 p = __ldcg(reinterpret_cast<const float4*>(&ps[lane + 32 * i]));
+        two[i] = Stats{p.x, p.y, p.z};
+      }
+      m = fmaxf(m, two[i].m);
+    }
+    m = warp_max(m);
+    st = warp_merge(two[0], m);
+#pragma unroll
+    for (uint32_t i = 1; i < kLpParts / 32; ++i) {
+      const Stats other = warp_merge(two[i], m);
+      st.s += other.s, st.w += other.w;
     }
     if (k) {
       // the k-th largest of the parts' first keys bounds the k-th largest key
-      const unsigned long long head = tid < a.splits ? __ldcg(&ps[tid].key[0]) : 0ull;
-      if (tid < a.splits) s_list[tid] = head;
+      if (tid < a.splits) s_list[tid] = head_key;
       if (tid == 0) s_key[0] = 0;
       __syncthreads();
       if (tid < a.splits && a.splits >= k) {
         uint32_t rank = 0;
-        for (uint32_t j = 0; j < a.splits; ++j) rank += s_list[j] > head;
-        if (rank == k - 1) s_key[0] = head;
+        for (uint32_t j = 0; j < a.splits; ++j) rank += s_list[j] > head_key;
+        if (rank == k - 1) s_key[0] = head_key;
       }
       __syncthreads();
       const unsigned long long t = s_key[0];
-      __syncthreads();
+      // at most k parts have a key from t up (or there are fewer than k parts): k * k <= kLpList entries
       for (uint32_t i = tid; i < a.splits * k; i += kLpThreads) {
         const unsigned long long key = __ldcg(&ps[i / k].key[i % k]);
         if (key != 0 && key >= t) s_list[atomicAdd(&s_n, 1u)] = key;
       }
       __syncthreads();
-      n_list = prune(s_list, s_n, k);
+      n_list = rank_list(s_list, s_n, k);
     }
   }
 
-  const float log_s = log2f(st.s);
+  const float log_s = kLn2 * log2f(st.s);
   const bool empty = st.s == 0.0f;  // nothing above -inf
-  const float lse = kLn2 * (st.m + log_s);
+  auto log_p = [&](float e) {
+    const float c = capped<kCap>(e, a);
+    return empty ? neg_inf() : c - st.m - log_s;
+  };
   if (tid == 0) {
-    a.entropy[row] = empty ? 0.0f : kLn2 * (log_s - st.w / st.s);
+    a.entropy[row] = empty ? 0.0f : log_s - kLn2 * (st.w / st.s);
     const int32_t tok = a.tokens[row];
     float lp = __int_as_float(0x7fc00000);
     if (tok >= 0 && (uint32_t)tok < a.V)
-      lp = empty ? neg_inf() : capped(Elem<T>::to(x[tok]), a.cap) - lse;
+      lp = log_p(Elem<T>::to(x[tok]));
     else if (tok >= 0)
       atomicOr(a.status, kStatusToken);
     a.logprob[row] = lp;
@@ -355,8 +475,40 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
     const unsigned long long key = s_list[tid];
     const uint64_t at = (uint64_t)row * k + tid;
     a.top_token[at] = (int32_t)(0xffffffffu - (uint32_t)key);
-    a.top_logprob[at] = empty ? neg_inf() : capped(of_ord((uint32_t)(key >> 32)), a.cap) - lse;
+    a.top_logprob[at] = log_p(of_ord((uint32_t)(key >> 32)));
   }
+}
+
+template <typename T>
+cudaError_t launch(LpArgs a, uint32_t rows, size_t work_bytes, uint32_t sms, cudaStream_t s) {
+  // Parts of a row: up to kLpTiles tiles each, fewer when that leaves SMs
+  // (4 CTAs each) without several rounds of work, at most kLpParts.
+  const uint32_t tile = kLpThreads * kLpVecs, n_vec = (uint32_t)((a.V * sizeof(T) + 15) / 16);
+  const uint32_t tiles = (n_vec + tile - 1) / tile;
+  uint64_t per = (uint64_t)tiles * rows / (kLpRounds * 4ull * sms);
+  per = per < 1 ? 1 : (per > kLpTiles ? kLpTiles : per);
+  const uint32_t least = (tiles + kLpParts - 1) / kLpParts;
+  if (per < least) per = least;
+  if (per > kLpTiles) return cudaErrorInvalidValue;  // V above kLpParts * kLpTiles tiles
+  a.splits = (tiles + (uint32_t)per - 1) / (uint32_t)per;
+  a.part_vecs = (tiles + a.splits - 1) / a.splits * tile;  // parts of one size
+  // rows of a launch: counters and parts fit the context's scratch
+  uint64_t batch = rows;
+  if (a.splits > 1) {
+    const uint64_t fit = work_bytes / (sizeof(LpPart) * a.splits);
+    batch = fit < kSplitCounters ? fit : kSplitCounters;
+  }
+  for (uint64_t done = 0; done < rows; done += batch) {
+    a.row0 = (uint32_t)done;
+    const uint32_t n = (uint32_t)(rows - done < batch ? rows - done : batch);
+    if (a.cap > 0.0f)
+      logprobs_kernel<T, true><<<n * a.splits, kLpThreads, 0, s>>>(a);
+    else
+      logprobs_kernel<T, false><<<n * a.splits, kLpThreads, 0, s>>>(a);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace
@@ -364,52 +516,48 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
 
 using namespace q4k;
 
-extern "C" int q4k_token_logprobs(q4k_ctx* ctx, uint32_t dtype, const void* logits, uint64_t stride, uint32_t rows,
-                                  uint32_t V, float cap, const int32_t* tokens, uint32_t top, float* logprob,
-                                  float* entropy, float* top_logprob, int32_t* top_token, void* stream) {
+extern "C" int q4k_token_logprobs(q4k_ctx* ctx, const q4k_logprobs_args* args, void* stream) {
   if (!ctx) return Q4K_ERR_INVALID_ARG;
-  if (dtype > Q4K_BF16) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: unknown dtype %u", dtype);
-  if (rows == 0) {
+  if (!args) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: null arguments");
+  const q4k_logprobs_args& x = *args;
+  if (x.dtype > Q4K_BF16) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: unknown dtype %u", x.dtype);
+  if (x.rows == 0) {
     ctx->err[0] = 0;
     return Q4K_OK;
   }
-  if (!logits || !tokens || !logprob || !entropy || (top && (!top_logprob || !top_token)))
+  if (!x.logits || !x.tokens || !x.logprob || !x.entropy || (x.top && (!x.top_logprob || !x.top_token)))
     return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: null pointer");
-  if (V == 0 || V >= (1u << 30) || rows >= (1u << 24))
-    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: V=%u or rows=%u out of range", V, rows);
-  if (top > kLpTop || top > V)
-    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: top=%u above %u or V=%u", top, kLpTop, V);
-  if (stride < V) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: stride below V=%u", V);
-  if (!(cap == cap)) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: cap is NaN");
-  if ((uintptr_t)logits % dtype_bytes(dtype))
+  if (x.V == 0 || x.V > kLpMaxV || x.rows >= (1u << 24))
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: V=%u or rows=%u out of range", x.V, x.rows);
+  if (x.top > kLpTop || x.top > x.V)
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: top=%u above %u or V=%u", x.top, kLpTop, x.V);
+  if (x.stride < x.V) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: stride below V=%u", x.V);
+  if (!(x.cap == x.cap)) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: cap is NaN");
+  if ((uintptr_t)x.logits % dtype_bytes(x.dtype))
     return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: logits not aligned to their type");
   LpArgs a{};
-  a.logits = logits;
-  a.stride = stride;
-  a.rows = rows;
-  a.V = V;
-  a.top = top;
-  a.cap = cap > 0.0f ? cap : 0.0f;
-  a.tokens = tokens;
-  a.logprob = logprob;
-  a.entropy = entropy;
-  a.top_logprob = top_logprob;
-  a.top_token = top_token;
+  a.logits = x.logits;
+  a.stride = x.stride;
+  a.V = x.V;
+  a.top = x.top;
+  a.cap = x.cap > 0.0f ? x.cap : 0.0f;
+  a.tokens = x.tokens;
+  a.logprob = x.logprob;
+  a.entropy = x.entropy;
+  a.top_logprob = x.top_logprob;
+  a.top_token = x.top_token;
   a.parts = reinterpret_cast<LpPart*>(ctx->xfrag);
   a.counters = ctx->split_counters;
   a.status = ctx->select.status;
-  // parts of a row: enough CTAs for every SM to hold several, no part below a tile
-  const uint32_t tile = kLpThreads * kLpVecs * 16 / (uint32_t)dtype_bytes(dtype);
-  const uint32_t want = (4 * (uint32_t)ctx->sm_count + rows - 1) / rows, most = (V + tile - 1) / tile;
-  a.splits = want < most ? want : most;
-  a.splits = a.splits > 64 ? 64 : a.splits;
-  if (rows > kSplitCounters || (uint64_t)rows * a.splits * sizeof(LpPart) > ctx->xfrag_cap) a.splits = 1;
+  a.cap_rate = a.cap > 0.0f ? 2.0f * kLog2e / a.cap : 0.0f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == Q4K_F32)
-    logprobs_kernel<float><<<rows * a.splits, kLpThreads, 0, st>>>(a);
-  else if (dtype == Q4K_F16)
-    logprobs_kernel<__half><<<rows * a.splits, kLpThreads, 0, st>>>(a);
+  const uint32_t sms = (uint32_t)ctx->sm_count;
+  cudaError_t e;
+  if (x.dtype == Q4K_F32)
+    e = launch<float>(a, x.rows, ctx->xfrag_cap, sms, st);
+  else if (x.dtype == Q4K_F16)
+    e = launch<__half>(a, x.rows, ctx->xfrag_cap, sms, st);
   else
-    logprobs_kernel<__nv_bfloat16><<<rows * a.splits, kLpThreads, 0, st>>>(a);
-  return ctx_cuda(ctx, cudaGetLastError(), "q4k_token_logprobs launch");
+    e = launch<__nv_bfloat16>(a, x.rows, ctx->xfrag_cap, sms, st);
+  return ctx_cuda(ctx, e, "q4k_token_logprobs launch");
 }

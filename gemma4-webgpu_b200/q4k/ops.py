@@ -11,6 +11,7 @@ call raises Q4KError.
 from __future__ import annotations
 
 import ctypes
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -74,9 +75,12 @@ class _KVCacheStruct(ctypes.Structure):  # q4k_kv_cache
                 ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32)]
 
 
-class _KVBatchStruct(ctypes.Structure):  # q4k_kv_batch
-    _fields_ = [("block_table", ctypes.c_void_p), ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
-                ("seqs", ctypes.c_uint32), ("tokens", ctypes.c_uint32), ("table_cols", ctypes.c_uint32)]
+# Argument records of include/q4k.h, packed in one call: a step issues these
+# operators once per layer, where a Python call's own time counts.
+_KV_BATCH = struct.Struct("<QQQIIIxxxx")  # q4k_kv_batch
+_KV_APPEND = struct.Struct("<QQQIIIxxxxQQQQQQQQQIIII")  # q4k_kv_batch, q4k_kv_append_args
+_ATTENTION = struct.Struct("<QQQIIIxxxxQQQQIIIIfxxxx")  # q4k_kv_batch, q4k_attention_args
+_LOGPROBS = struct.Struct("<QQQQQQQIIIIfxxxx")  # q4k_logprobs_args
 
 
 class KVCache:
@@ -106,7 +110,7 @@ class KVCache:
         self.device = k.device
         self._struct = _KVCacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, page,
                                       heads, dim)
-        self._ref = ctypes.byref(self._struct)
+        self._addr = ctypes.addressof(self._struct)
 
     @classmethod
     def allocate(cls, pages: int, kv_heads: int, page_size: int, head_dim: int,
@@ -140,6 +144,8 @@ class Context:
         if rc != _lib.Q4K_OK:
             raise Q4KError(rc, f"q4k_create(device={self.device.index}) failed")
         self._h = handle.value
+        self._args = bytearray(256)  # the argument record of the call being made
+        self._args_addr = ctypes.addressof((ctypes.c_char * 256).from_buffer(self._args))
 
     def close(self) -> None:
         if getattr(self, "_h", None):
@@ -431,35 +437,45 @@ class Context:
 
     # ---- cached attention (see include/q4k.h) ----------------------------------
 
+    def _current_stream(self, stream: torch.cuda.Stream | None) -> int:
+        if stream is not None:
+            return stream.cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.device.index)  # no Stream object for the common call
+
     def _rows(self, t: torch.Tensor, name: str, dtype: torch.dtype, tokens: int, dim: int) -> tuple[int, int]:
         """(heads, row stride) of rows [tokens, heads, head_dim]: any row stride, heads side by side."""
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor")
-        if t.device != self.device:
+        if t.get_device() != self.device.index:
             raise ValueError(f"{name} is on {t.device}, expected {self.device}")
-        if t.dtype != dtype:
+        if t.dtype is not dtype:
             raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
-        shape, stride = t.shape, t.stride()
+        shape = t.shape
         if len(shape) != 3 or shape[0] != tokens or shape[2] != dim:
             raise ValueError(f"{name} must be [{tokens}, heads, {dim}]")
-        if stride[2] != 1 or (stride[1] != dim and shape[1] > 1):
+        row, head, one = t.stride()
+        heads = shape[1]
+        if one != 1 or (head != dim and heads > 1):
             raise ValueError(f"{name}: the heads of a row must be contiguous")
-        return shape[1], stride[0] if tokens > 1 else shape[1] * dim
+        return heads, row if tokens > 1 else heads * dim
 
-    def _batch(self, cache: KVCache, tokens: int, block_table: torch.Tensor, q_start: torch.Tensor,
-               kv_len: torch.Tensor):
+    def _need_batch(self, cache: KVCache, block_table: torch.Tensor, q_start: torch.Tensor,
+                    kv_len: torch.Tensor) -> tuple[int, int]:
+        """(sequences, block table columns)."""
         if not isinstance(cache, KVCache):
             raise TypeError("cache must be a KVCache")
-        if cache.device != self.device:
-            raise ValueError(f"cache is on {cache.device}, expected {self.device}")
-        _need(block_table, torch.int32, "block_table", self.device)
-        _need(q_start, torch.int32, "q_start", self.device)
-        _need(kv_len, torch.int32, "kv_len", self.device)
+        index = self.device.index
+        if cache.k.get_device() != index:
+            raise ValueError(f"cache is on {cache.k.device}, expected {self.device}")
+        for t, name in ((block_table, "block_table"), (q_start, "q_start"), (kv_len, "kv_len")):
+            if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == index
+                    and t.is_contiguous()):
+                _need(t, torch.int32, name, self.device)
         seqs = kv_len.numel()
-        if block_table.dim() != 2 or block_table.shape[0] != seqs or q_start.numel() != seqs + 1:
+        shape = block_table.shape
+        if len(shape) != 2 or shape[0] != seqs or q_start.numel() != seqs + 1:
             raise ValueError("block_table must be [seqs, columns], q_start [seqs + 1] and kv_len [seqs]")
-        return ctypes.byref(_KVBatchStruct(block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), seqs, tokens,
-                                           block_table.shape[1]))
+        return seqs, shape[1]
 
     def kv_append(self, cache: KVCache, k: torch.Tensor, v: torch.Tensor, rope: torch.Tensor | None,
                   block_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
@@ -471,19 +487,24 @@ class Context:
         None for no rotation.  kv_len counts the new tokens.  With q
         [tokens, q_heads, head_dim] the queries are rotated in the same launch
         and returned (q_out, which may be q)."""
+        seqs, cols = self._need_batch(cache, block_table, q_start, kv_len)
+        if not isinstance(k, torch.Tensor):
+            raise TypeError("k must be a torch.Tensor")
         tokens, dim, dtype = k.shape[0], cache.head_dim, k.dtype
-        if dtype not in DTYPES:
+        code = DTYPES.get(dtype)
+        if code is None:
             raise TypeError(f"k has dtype {dtype}, expected one of {tuple(DTYPES)}")
         heads, k_stride = self._rows(k, "k", dtype, tokens, dim)
         v_heads, v_stride = self._rows(v, "v", dtype, tokens, dim)
-        if heads != cache.kv_heads or v_heads != cache.kv_heads:
+        if heads != cache.kv_heads or v_heads != heads:
             raise ValueError(f"k and v must have the cache's {cache.kv_heads} heads")
-        rope_len = rope_dim = q_heads = q_stride = qo_stride = 0
+        rope_len = rope_dim = rope_ptr = q_heads = q_stride = qo_stride = q_ptr = qo_ptr = 0
         if rope is not None:
             _need(rope, torch.float32, "rope", self.device)
-            if rope.dim() != 3 or rope.shape[2] != 2:
+            shape = rope.shape
+            if len(shape) != 3 or shape[2] != 2:
                 raise ValueError("rope must be [positions, pairs, 2]")
-            rope_len, rope_dim = rope.shape[0], 2 * rope.shape[1]
+            rope_len, rope_dim, rope_ptr = shape[0], 2 * shape[1], rope.data_ptr()
         if q is not None:
             q_heads, q_stride = self._rows(q, "q", dtype, tokens, dim)
             if q_out is None:
@@ -491,10 +512,14 @@ class Context:
             qo_heads, qo_stride = self._rows(q_out, "q_out", dtype, tokens, dim)
             if qo_heads != q_heads:
                 raise ValueError("q_out and q differ in shape")
-        self._check(self._L.q4k_kv_append(
-            self._h, cache._ref, self._batch(cache, tokens, block_table, q_start, kv_len), DTYPES[dtype], _ptr(k),
-            k_stride, _ptr(v), v_stride, _ptr(rope), rope_len, rope_dim, _ptr(q), q_stride,
-            _ptr(q_out) if q is not None else None, qo_stride, q_heads, _stream(stream)))
+            q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
+        _KV_APPEND.pack_into(self._args, 0, block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), seqs, tokens,
+                             cols, k.data_ptr(), v.data_ptr(), q_ptr, qo_ptr, rope_ptr, k_stride, v_stride, q_stride,
+                             qo_stride, code, q_heads, rope_len, rope_dim)
+        addr = self._args_addr
+        rc = self._L.q4k_kv_append(self._h, cache._addr, addr, addr + _KV_BATCH.size, self._current_stream(stream))
+        if rc:
+            self._check(rc)
         return q_out if q is not None else None
 
     def paged_attention(self, cache: KVCache, q: torch.Tensor, block_table: torch.Tensor, q_start: torch.Tensor,
@@ -505,20 +530,29 @@ class Context:
         position kv_len - n + i and sees the positions up to its own, the last
         `window` of them when window > 0; a row that sees none is zero.  max_q:
         the most new rows of one sequence, known on the host."""
+        seqs, cols = self._need_batch(cache, block_table, q_start, kv_len)
+        if not isinstance(q, torch.Tensor):
+            raise TypeError("q must be a torch.Tensor")
         tokens, dim, dtype = q.shape[0], cache.head_dim, q.dtype
-        if dtype not in DTYPES:
+        code = DTYPES.get(dtype)
+        if code is None:
             raise TypeError(f"q has dtype {dtype}, expected one of {tuple(DTYPES)}")
         heads, q_stride = self._rows(q, "q", dtype, tokens, dim)
-        if window < 0 or max_q < 0:
-            raise ValueError("window and max_q must not be negative")
+        if not (0 <= window < 1 << 31 and 0 <= max_q < 1 << 31):
+            raise ValueError("window and max_q must lie in 0 .. 2^31 - 1")
         if out is None:
             out = torch.empty((tokens, heads, dim), dtype=dtype, device=self.device)
         out_heads, out_stride = self._rows(out, "out", dtype, tokens, dim)
         if out_heads != heads:
             raise ValueError("out and q differ in shape")
-        self._check(self._L.q4k_paged_attention(
-            self._h, cache._ref, self._batch(cache, tokens, block_table, q_start, kv_len), DTYPES[dtype], _ptr(q),
-            q_stride, _ptr(out), out_stride, heads, max_q, scale, window, _stream(stream)))
+        _ATTENTION.pack_into(self._args, 0, block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), seqs, tokens,
+                             cols, q.data_ptr(), out.data_ptr(), q_stride, out_stride, code, heads, max_q, window,
+                             scale)
+        addr = self._args_addr
+        rc = self._L.q4k_paged_attention(self._h, cache._addr, addr, addr + _KV_BATCH.size,
+                                         self._current_stream(stream))
+        if rc:
+            self._check(rc)
         return out
 
     # ---- token log probabilities ---------------------------------------------------
@@ -534,26 +568,31 @@ class Context:
         entropy [rows], top_logprob [rows, top], top_token int32 [rows, top])."""
         if not isinstance(logits, torch.Tensor):
             raise TypeError("logits must be a torch.Tensor")
-        if logits.device != self.device:
+        if logits.get_device() != self.device.index:
             raise ValueError(f"logits is on {logits.device}, expected {self.device}")
-        if logits.dtype not in DTYPES:
+        code = DTYPES.get(logits.dtype)
+        if code is None:
             raise TypeError(f"logits has dtype {logits.dtype}, expected one of {tuple(DTYPES)}")
-        if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        if logits.dim() != 2:
+            raise ValueError("logits must be [rows, V] with contiguous rows")
+        rows, V = logits.shape
+        row, one = logits.stride()
+        if one != 1 and V > 1:
             raise ValueError("logits must be [rows, V] with contiguous rows")
         _need(tokens, torch.int32, "tokens", self.device)
-        rows, V = logits.shape
         if tokens.numel() != rows:
             raise ValueError("tokens must hold one id for each row")
-        if top < 0 or top > min(32, V):
+        if not 0 <= top <= min(32, V):
             raise ValueError("top must lie in 0..32 and not exceed V")
-        stats = torch.empty((2, rows), dtype=torch.float32, device=self.device)
-        top_logprob = torch.empty((rows, top), dtype=torch.float32, device=self.device)
-        top_token = torch.empty((rows, top), dtype=torch.int32, device=self.device)
-        logprob, entropy = stats.unbind(0)
-        self._check(self._L.q4k_token_logprobs(
-            self._h, DTYPES[logits.dtype], _ptr(logits), logits.stride(0) if rows > 1 else V, rows, V, cap,
-            _ptr(tokens), top, _ptr(logprob), _ptr(entropy), _ptr(top_logprob) if top else None,
-            _ptr(top_token) if top else None, _stream(stream)))
+        top_token = tokens.new_empty((rows, top))
+        like = logits if code == 0 else tokens.new_empty(0, dtype=torch.float32)
+        logprob, entropy, top_logprob = like.new_empty(rows), like.new_empty(rows), like.new_empty((rows, top))
+        _LOGPROBS.pack_into(self._args, 0, logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(),
+                            top_logprob.data_ptr(), top_token.data_ptr(), row if rows > 1 else V, code, rows, V, top,
+                            cap)
+        rc = self._L.q4k_token_logprobs(self._h, self._args_addr, self._current_stream(stream))
+        if rc:
+            self._check(rc)
         return logprob, entropy, top_logprob, top_token
 
     def exchange(self, rank: int, world: int) -> "Exchange":

@@ -364,53 +364,86 @@ typedef struct {
   uint32_t table_cols;
 } q4k_kv_batch;
 
-/* Append the batch's new keys and values (k, v: rows of kv_heads * head_dim
- * elements of `dtype`, `*_stride` elements apart) to the cache.  Keys are
- * rotated by their positions first: pairs (j, j + rope_dim/2) of the first
- * rope_dim elements of a head by rope[position][j] = (cos, sin), a
- * [rope_len][rope_dim/2][2] table (rope_dim = 0: no rotation; the pairing of
- * shaders/rope.wgsl:14-20; store as shaders/kv_cache_store.wgsl).  With q (may
- * be NULL) the batch's queries, q_heads a row, are rotated into q_out in the
- * same launch (q_out may be q).  A block's scale is the smallest power of two
- * that holds its largest magnitude; it grows as tokens arrive and the codes
- * already there are rescaled, so the order and size of the appends do not
- * matter (but for e4m3's subnormal range).  Infinities are stored as the
- * block's largest code and NaN as zero, and q4k_check then returns
- * Q4K_ERR_INVALID_ARG. */
-Q4K_API int q4k_kv_append(q4k_ctx* ctx, const q4k_kv_cache* cache, const q4k_kv_batch* batch, uint32_t dtype,
-                          const void* k, uint64_t k_stride, const void* v, uint64_t v_stride, const float* rope,
-                          uint32_t rope_len, uint32_t rope_dim, const void* q, uint64_t q_stride, void* q_out,
-                          uint64_t q_out_stride, uint32_t q_heads, void* stream);
+typedef struct {
+  const void* k;       /* [tokens] rows of kv_heads * head_dim elements of `dtype` */
+  const void* v;
+  const void* q;       /* [tokens] rows of q_heads * head_dim, or NULL */
+  void* q_out;         /* the rotated queries; may be q */
+  const float* rope;   /* [rope_len][rope_dim / 2][2]: (cos, sin) of a position and pair */
+  uint64_t k_stride;   /* elements from row to row */
+  uint64_t v_stride;
+  uint64_t q_stride;
+  uint64_t q_out_stride;
+  uint32_t dtype;      /* Q4K_F32, Q4K_F16 or Q4K_BF16: k, v, q, q_out */
+  uint32_t q_heads;
+  uint32_t rope_len;   /* positions of the table */
+  uint32_t rope_dim;   /* rotated elements of a head, a multiple of 16; 0: no rotation */
+} q4k_kv_append_args;
+
+/* Append the batch's new keys and values to the cache.  Keys are rotated by
+ * their positions first: pairs (j, j + rope_dim/2) of the first rope_dim
+ * elements of a head by rope[position][j] (the pairing of
+ * shaders/rope.wgsl:14-20; store as shaders/kv_cache_store.wgsl).  With q the
+ * batch's queries are rotated into q_out in the same launch.  A block's scale
+ * is the smallest power of two that holds its largest magnitude; it grows as
+ * tokens arrive and the codes already there are rescaled, so the order and
+ * size of the appends do not matter (but for e4m3's subnormal range).
+ * Infinities are stored as the block's largest code and NaN as zero, and
+ * q4k_check then returns Q4K_ERR_INVALID_ARG.  Rows: 16-byte aligned. */
+Q4K_API int q4k_kv_append(q4k_ctx* ctx, const q4k_kv_cache* cache, const q4k_kv_batch* batch,
+                          const q4k_kv_append_args* args, void* stream);
+
+typedef struct {
+  const void* q;       /* [tokens] rows of q_heads * head_dim elements of `dtype` */
+  void* out;           /* the same layout */
+  uint64_t q_stride;   /* elements from row to row */
+  uint64_t out_stride;
+  uint32_t dtype;
+  uint32_t q_heads;    /* 1..64 times kv_heads; head h reads key head h / (q_heads / kv_heads) */
+  uint32_t max_q;      /* largest number of new rows of one sequence: a hint that selects kernels */
+  uint32_t window;     /* 0: none */
+  float scale;
+} q4k_attention_args;
 
 /* Causal attention of the batch's rows over the cache: out[r][h] =
  * sum_j softmax_j(scale * q[r][h] . k[j]) v[j] over the positions j of the
  * row's sequence up to its own, the last `window` of them when window > 0
- * (shaders/attn_score.wgsl:14-39, softmax.wgsl, attn_output.wgsl:10-22);
- * head h reads key head h / (q_heads / kv_heads).  A row that sees no
- * position is zero.  q, out: rows of q_heads * head_dim elements of `dtype`.
- * f32 rows are computed to f32 accuracy, f16 and bf16 rows to that of their
- * type, sums and softmax statistics in f32 for all.  max_q: the largest
- * number of new rows of one sequence, a hint that selects kernels.  Uses the
- * context's scratch: order the calls of one context on one stream. */
-Q4K_API int q4k_paged_attention(q4k_ctx* ctx, const q4k_kv_cache* cache, const q4k_kv_batch* batch, uint32_t dtype,
-                                const void* q, uint64_t q_stride, void* out, uint64_t out_stride, uint32_t q_heads,
-                                uint32_t max_q, float scale, uint32_t window, void* stream);
+ * (shaders/attn_score.wgsl:14-39, softmax.wgsl, attn_output.wgsl:10-22).  A
+ * row that sees no position is zero.  f32 rows are computed to f32 accuracy,
+ * f16 and bf16 rows to that of their type, sums and softmax statistics in
+ * f32 for all.  Uses the context's scratch: order the calls of one context
+ * on one stream. */
+Q4K_API int q4k_paged_attention(q4k_ctx* ctx, const q4k_kv_cache* cache, const q4k_kv_batch* batch,
+                                const q4k_attention_args* args, void* stream);
 
-/* For each of `rows` rows of V logits (of `dtype`, `stride` elements apart):
- * x = cap > 0 ? cap * tanh(logit / cap) : logit (shaders/logit_softcap.wgsl),
- *   logprob = x[token] - log sum exp x           (NaN for token < 0: none)
+typedef struct {
+  const void* logits;     /* [rows] rows of V elements of `dtype` */
+  const int32_t* tokens;  /* [rows] */
+  float* logprob;         /* [rows] */
+  float* entropy;         /* [rows] */
+  float* top_logprob;     /* [rows][top]; may be NULL with top = 0 */
+  int32_t* top_token;     /* [rows][top] */
+  uint64_t stride;        /* elements from row to row */
+  uint32_t dtype;
+  uint32_t rows;
+  uint32_t V;
+  uint32_t top;           /* 0..32 */
+  float cap;              /* <= 0: none */
+} q4k_logprobs_args;
+
+/* For each row of logits:
+ *   x = cap > 0 ? cap * tanh(logit / cap) : logit  (shaders/logit_softcap.wgsl)
+ *   logprob = x[token] - log sum exp x            (NaN for token < 0: none)
  *   entropy = -sum p log p, p = softmax(x)
- *   top_token / top_logprob [rows][top]: the `top` (0..32) largest logits in
- * descending order, ties to the lower index, NaN last, and their
- * log probabilities.  Sums in f32.  A token >= V gives NaN and q4k_check
- * returns Q4K_ERR_INVALID_ARG.  A row with a NaN or +inf has NaN statistics;
- * one with nothing above -inf has log probabilities of -inf and entropy 0.
- * The reference samples from 256 raw candidates on the host
- * (src/engine.ts:1792-1837) and has no log probabilities.  Uses the
- * context's scratch: order the calls of one context on one stream. */
-Q4K_API int q4k_token_logprobs(q4k_ctx* ctx, uint32_t dtype, const void* logits, uint64_t stride, uint32_t rows,
-                               uint32_t V, float cap, const int32_t* tokens, uint32_t top, float* logprob,
-                               float* entropy, float* top_logprob, int32_t* top_token, void* stream);
+ *   top_token, top_logprob: the `top` largest logits in descending order,
+ *     ties to the lower index, NaN last, and their log probabilities.
+ * Sums in f32.  A token >= V gives NaN and q4k_check returns
+ * Q4K_ERR_INVALID_ARG.  A row with a NaN or +inf has NaN statistics; one with
+ * nothing above -inf has log probabilities of -inf and entropy 0.  The
+ * reference samples from 256 raw candidates on the host
+ * (src/engine.ts:1792-1837) and has no log probabilities.  Uses the context's
+ * scratch: order the calls of one context on one stream. */
+Q4K_API int q4k_token_logprobs(q4k_ctx* ctx, const q4k_logprobs_args* args, void* stream);
 
 /* ---- the chained decode step -------------------------------------------
  * One token's layers as a true chain, each layer reading the previous

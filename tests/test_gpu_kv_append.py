@@ -207,7 +207,7 @@ def test_refusals(ctx):
         (dict(k=kd.double()), TypeError), (dict(v=vd.half()), TypeError), (dict(k=kd[:, :, :32]), ValueError),
         (dict(v=vd[:2]), ValueError), (dict(rope=rd[:, :, :1]), ValueError), (dict(rope=rd[:, :5].contiguous()), q4k.Q4KError),
         (dict(q_start=qs.long()), TypeError), (dict(q_start=qs[:1]), ValueError), (dict(block_table=table[0]), ValueError),
-        (dict(kv_len=kvl.cpu()), ValueError), (dict(cache=None), AttributeError), (dict(q=qd, q_out=qd[:, :1]), ValueError),
+        (dict(kv_len=kvl.cpu()), ValueError), (dict(cache=None), TypeError), (dict(q=qd, q_out=qd[:, :1]), ValueError),
         (dict(k=torch.zeros(3, 1, 65, device=DEV)[:, :, 1:]), q4k.Q4KError),  # rows not 16-byte aligned
     ]
     for change, err in bad:
