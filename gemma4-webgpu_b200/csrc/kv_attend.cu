@@ -39,18 +39,29 @@ namespace q4k {
 namespace {
 
 constexpr float kPShift = 14.0f;  // probabilities are stored times 2^14: f16 then holds them down to 2^-28 in full
-constexpr uint32_t kMergeGroup = 16;
+constexpr uint32_t kMergeGroup = 24;  // most parts one CTA merges at a time; its square covers every grid
+static_assert(kMergeGroup * kMergeGroup >= kAttendMaxCtas, "two levels of merging");
 
-template <int D>
+// Copies run two blocks ahead, keys and values on their own: a slot is free
+// again after its product.  At head dim 512 a warp has two key slots and one
+// value slot, whose copy then overlaps the next block's scores: 8 warps (two a
+// scheduler, which the arithmetic needs: 4 ran at 70% of it) fit shared memory.
+template <int D, int NT>
 struct AttendCfg {
-  static constexpr int kWarps = D == 512 ? 4 : 8;
-  static constexpr int kCtas = 1;                        // CTAs an SM
-  static constexpr int kStages = D >= 256 ? 3 : 4;
+  static constexpr int kWarps = 8;
+  static constexpr int kCtas = D <= 64 || (D == 128 && NT == 1) ? 2 : 1;  // CTAs an SM: one streams while another starts or ends a unit
+  static constexpr int kKSlots = 2, kVSlots = D == 512 ? 1 : 2;
+  static constexpr int kVAhead = D == 512 ? 1 : 2;       // blocks that value copies run ahead
+  static constexpr int kKWait = D == 512 ? 2 : 3;        // copy groups that may be pending when a block's keys are read
+  static constexpr int kVWait = D == 512 ? 1 : 3;        // ... its values
   static constexpr int kRow = D + 16;                    // bytes of a staged row: the pad spreads rows over the banks
-  static constexpr int kStage = 2 * 16 * kRow + 16;      // 16 keys, 16 values, their scales
-  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kSlot = 16 * kRow + 16;           // 16 keys or values and their scale
+  static constexpr int kRing = kWarps * (kKSlots + kVSlots) * kSlot;
   static constexpr int kVec = D >= 128 ? 16 : 8;         // bytes of a value row a thread takes at a time
   static constexpr int kPasses = D / (8 * kVec);         // value passes of 8 threads x kVec bytes
+  // What a unit's start costs, in 16-key blocks of a CTA's time: the ranges
+  // count it, so that CTAs with two units get fewer blocks.
+  static constexpr uint32_t kStart = D >= 256 ? 16 : 8;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -108,9 +119,10 @@ __device__ __forceinline__ uint32_t piece(uint32_t row, uint32_t u) {
 struct Seg {  // a sequence's share of the work
   KvSeq s;
   uint32_t first, blocks, groups;  // first 16-key block, blocks, row groups
+  uint32_t cost;                   // of a unit: its blocks and its start
 };
 
-template <int R>
+template <int R, uint32_t kStart>
 __device__ __forceinline__ Seg seq_work(const AttendArgs& a, uint32_t b) {
   Seg w;
   w.s = kv_seq(a.b, a.c.page_shift, b);
@@ -120,12 +132,13 @@ __device__ __forceinline__ Seg seq_work(const AttendArgs& a, uint32_t b) {
   const int low = a.window ? (int)w.s.kv - (int)w.s.n - (int)a.window + 1 : 0;
   w.first = low > 0 ? (uint32_t)low / 16 : 0;
   w.blocks = (w.s.kv + 15) / 16 - min(w.first, (w.s.kv + 15) / 16);
+  w.cost = w.blocks ? w.blocks + kStart : 0;
   return w;
 }
 
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas) attend_kernel(const AttendArgs a) {
-  using C = AttendCfg<D>;
+__global__ void __launch_bounds__(AttendCfg<D, NT>::kWarps * 32, AttendCfg<D, NT>::kCtas) attend_kernel(const AttendArgs a) {
+  using C = AttendCfg<D, NT>;
   constexpr bool kHiLo = Elem<T>::kExact;
   constexpr int R = 8 * NT;  // rows of a unit
   constexpr int kThreads = C::kWarps * 32;
@@ -133,7 +146,7 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas
   extern __shared__ __align__(16) uint8_t smem[];
   uint8_t* const ring = smem;
   uint8_t* const qf = smem + C::kRing;  // [D / 16][NT][32 lanes] row operand in fragment order
-  __shared__ float s_rs[R], s_m[C::kWarps][R], s_l[C::kWarps][R], s_f[2 * kMergeGroup][R], s_tot[R];
+  __shared__ float s_rs[R], s_m[C::kWarps][R], s_l[C::kWarps][R], s_f[kMergeGroup][R], s_pl[kMergeGroup][R], s_tot[R];
   __shared__ uint32_t s_scan[C::kWarps + 1];
   __shared__ uint32_t s_off, s_seq, s_last;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
@@ -146,8 +159,8 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas
   uint32_t mine = 0;
   bool none = false;  // a sequence with rows that see nothing, or one that cannot be served
   for (uint32_t b = b_lo; b < b_hi; ++b) {
-    const Seg w = seq_work<R>(a, b);
-    mine += w.blocks * w.groups * H;  // 2^32 blocks would be 4 TB of the smallest cache
+    const Seg w = seq_work<R, C::kStart>(a, b);
+    mine += w.cost * w.groups * H;  // 2^32 blocks would be 4 TB of the smallest cache
     none |= w.s.bad || (w.groups && w.blocks == 0);
   }
   uint32_t scan = mine;
@@ -160,7 +173,7 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas
   if (tid == 0) s_scan[0] = 0;
   if (__syncthreads_or(none)) {
     for (uint32_t b = blockIdx.x; b < a.b.seqs; b += gridDim.x) {
-      const Seg w = seq_work<R>(a, b);
+      const Seg w = seq_work<R, C::kStart>(a, b);
       if (w.s.bad && tid == 0) atomicOr(a.status, kStatusKvMeta);
       if (w.groups && w.blocks == 0) {
         const uint32_t per = H * G * D;
@@ -185,8 +198,8 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas
   if (cur >= before && cur < before + mine) {
     uint32_t o = before;
     for (uint32_t b = b_lo; b < b_hi; ++b) {
-      const Seg w = seq_work<R>(a, b);
-      const uint32_t c = w.blocks * w.groups * H;
+      const Seg w = seq_work<R, C::kStart>(a, b);
+      const uint32_t c = w.cost * w.groups * H;
       if (cur < o + c) {
         s_seq = b;
         s_off = o;
@@ -200,102 +213,116 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas
   uint32_t seq0 = s_off;  // global index of sequence b's first block
 
   const uint32_t row_k = (g >> 1) + 4 * (g & 1);  // the key (of 8) that fragment row g holds: conflict-free with kRow
-  const uint32_t ring_u = smem_u32(ring) + warp * C::kStages * C::kStage;
+  uint8_t* const k_ring = ring + warp * (C::kKSlots + C::kVSlots) * C::kSlot;  // this warp's slots
+  uint8_t* const v_ring = k_ring + C::kKSlots * C::kSlot;
 
   while (cur < end) {
-    const Seg w = seq_work<R>(a, b);
-    const uint32_t cnt = w.blocks * w.groups * H;
+    const Seg w = seq_work<R, C::kStart>(a, b);
+    const uint32_t cnt = w.cost * w.groups * H;
     if (cur >= seq0 + cnt) {
       seq0 += cnt;
       ++b;
       continue;
     }
-    const uint32_t unit = (cur - seq0) / w.blocks, u_off = (cur - seq0) % w.blocks;
+    // the first kStart places of a unit stand for its start, the others for its blocks
+    const uint32_t unit = (cur - seq0) / w.cost, u0 = seq0 + unit * w.cost;
+    const uint32_t stop = min(end, u0 + w.cost);
+    if (stop <= u0 + C::kStart) {  // nothing but a start: the next CTA has the unit
+      cur = stop;
+      continue;
+    }
+    const uint32_t u_off = max(cur, u0 + C::kStart) - (u0 + C::kStart), n_blk = stop - (u0 + C::kStart) - u_off;
     const uint32_t h = unit / w.groups, rg = unit % w.groups;
-    const uint32_t n_blk = min(w.blocks - u_off, end - cur);
     const uint32_t blk0 = w.first + u_off;
     const uint32_t row0 = rg * R, n_rows = min((uint32_t)R, w.s.n * G - row0);
     const int pos0 = (int)w.s.kv - (int)w.s.n;
 
+    // ---- the rows, before the copies that would delay them ---------------------
+    constexpr int kChunks = D >= 128 ? D / 128 : 1, kMine = (R + C::kWarps - 1) / C::kWarps;
+    float x[kMine][kChunks][4];
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {  // every load is on its way before the first is used
+      const uint32_t r = warp + k * C::kWarps, rr = row0 + r;
+      const T* src = static_cast<const T*>(a.q) + (uint64_t)(w.s.t0 + rr / G) * a.q_stride + (h * G + rr % G) * D;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        x[k][i][0] = x[k][i][1] = x[k][i][2] = x[k][i][3] = 0.0f;
+        if (r < n_rows && lane * 4 < (uint32_t)D) load_elems(src + 128 * i + 4 * lane, x[k][i]);
+      }
+    }
     // ---- the copy ring: warp w takes blocks blk0 + w, + kWarps, ... -----------
     const uint32_t n_mine = n_blk > warp ? (n_blk - warp + C::kWarps - 1) / C::kWarps : 0;
     const uint32_t* const table = a.b.table + (uint64_t)b * a.b.cols;
     auto page_of = [&](uint32_t i) {
       return i < n_mine ? table[((blk0 + warp + i * C::kWarps) * 16) >> a.c.page_shift] : 0u;
     };
-    auto issue = [&](uint32_t i, uint32_t page) {
+    auto issue = [&](uint32_t i, uint32_t page, bool value) {
       if (i < n_mine) {
         const uint32_t pos = (blk0 + warp + i * C::kWarps) * 16;
         uint64_t blk;
-        bool ok = kv_block(a.c, page, h, pos, &blk);
+        const bool ok = kv_block(a.c, page, h, pos, &blk);
         if (!ok) {  // out of range: read nothing (zeros), report
           if (lane == 0) atomicOr(a.status, kStatusKvMeta);
           blk = 0;
         }
-        const uint32_t st = ring_u + (i % C::kStages) * C::kStage;
-        const uint8_t* ks = a.c.k + blk * (16 * D);
-        const uint8_t* vs = a.c.v + blk * (16 * D);
-        // slots past the sequence's end are read as zeros, whatever they hold
+        const uint32_t st = smem_u32(value ? v_ring + (i % C::kVSlots) * C::kSlot : k_ring + (i % C::kKSlots) * C::kSlot);
+        const uint8_t* src = (value ? a.c.v : a.c.k) + blk * (16 * D);
+        // slots past the end are read as zeros, whatever they hold
         const uint32_t rows = ok ? min(16u, w.s.kv - pos) : 0u;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
           const uint32_t c = lane + 32 * j, r = c / (D / 16), x = c % (D / 16);
-          cp_async16(st + r * C::kRow + 16 * x, ks + 16 * c, r < rows);
-          cp_async16(st + 16 * C::kRow + r * C::kRow + 16 * x, vs + 16 * c, r < rows);
+          cp_async16(st + r * C::kRow + 16 * x, src + 16 * c, r < rows);
         }
-        if (lane < 2) cp_async4(st + 32 * C::kRow + 4 * lane, (lane ? a.c.vs : a.c.ks) + blk);
+        if (lane == 0) cp_async4(st + 16 * C::kRow, (value ? a.c.vs : a.c.ks) + blk);
       }
       cp_commit();
     };
-    uint32_t page_next = page_of(0);
-#pragma unroll
-    for (int i = 0; i < C::kStages - 1; ++i) {
-      const uint32_t p = page_next;
-      page_next = page_of(i + 1);
-      issue(i, p);
+    uint32_t page1 = page_of(1), page2 = page_of(2);  // of the next two blocks
+    {
+      const uint32_t page0 = page_of(0);
+      issue(0, page0, false);
+      issue(0, page0, true);
+      issue(1, page1, false);
+      if (C::kVAhead == 2) issue(1, page1, true);
     }
 
     // ---- the rows' operand: f16 (hi, lo) fragments under a power of two per row
-    for (uint32_t r = warp; r < (uint32_t)R; r += C::kWarps) {
-      float x[D / 32 < 4 ? 1 : D / 128][4];
-      float mx = 0.0f;
-      const uint32_t rr = row0 + r;
-      const T* src = static_cast<const T*>(a.q) + (uint64_t)(w.s.t0 + rr / G) * a.q_stride + (h * G + rr % G) * D;
-      constexpr int kChunks = D >= 128 ? D / 128 : 1;
+    {
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        if (r < n_rows && lane * 4 < (uint32_t)D) {
-          load_elems(src + 128 * i + 4 * lane, x[i]);
-        } else {
-          x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
+      for (int k = 0; k < kMine; ++k) {
+        const uint32_t r = warp + k * C::kWarps;
+        if (R % C::kWarps && r >= (uint32_t)R) break;
+        float mx = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float v = fabsf(x[k][i][j]);
+            if (v <= 3.402823466e38f) mx = fmaxf(mx, v);
+          }
+        const uint32_t mb = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
+        int e = 13 - ((int)(mb >> 23) - 127);  // the largest element in [2^13, 2^14)
+        e = mb == 0 ? 0 : min(max(e, -110), 110);
+        const float up = exp2i(e);
+        if (lane == 0) s_rs[r] = a.scale_log2 * exp2i(-e);
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+          const uint32_t d = 128 * i + 4 * lane;
+          if (d >= (uint32_t)D) break;
+          float v[4], lo[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            v[j] = x[k][i][j] * up;
+            lo[j] = v[j] - __half2float(__float2half_rn(v[j]));
+          }
+          // dims d..d+3 are one thread's four of k-step (d / 64, (d % 16) / 4)
+          const uint32_t step = (d / 64) * 4 + (d % 16) / 4, ln = (r % 8) * 4 + (d % 64) / 16;
+          uint8_t* dst = qf + (step * NT + r / 8) * kQStep + ln * (kHiLo ? 16 : 8);
+          *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f16(v[0], v[1]), pack_f16(v[2], v[3]));
+          if constexpr (kHiLo)
+            *reinterpret_cast<uint2*>(dst + 8) = make_uint2(pack_f16(lo[0], lo[1]), pack_f16(lo[2], lo[3]));
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float v = fabsf(x[i][j]);
-          if (v <= 3.402823466e38f) mx = fmaxf(mx, v);
-        }
-      }
-      const uint32_t mb = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
-      int e = 13 - ((int)(mb >> 23) - 127);  // the largest element in [2^13, 2^14)
-      e = mb == 0 ? 0 : min(max(e, -110), 110);
-      const float up = exp2i(e);
-      if (lane == 0) s_rs[r] = a.scale_log2 * exp2i(-e);
-#pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const uint32_t d = 128 * i + 4 * lane;
-        if (d >= (uint32_t)D) break;
-        float v[4], lo[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[j] = x[i][j] * up;
-          lo[j] = v[j] - __half2float(__float2half_rn(v[j]));
-        }
-        // dims d..d+3 are one thread's four of k-step (d / 64, (d % 16) / 4)
-        const uint32_t step = (d / 64) * 4 + (d % 16) / 4, ln = (r % 8) * 4 + (d % 64) / 16;
-        uint8_t* dst = qf + (step * NT + r / 8) * kQStep + ln * (kHiLo ? 16 : 8);
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f16(v[0], v[1]), pack_f16(v[2], v[3]));
-        if constexpr (kHiLo)
-          *reinterpret_cast<uint2*>(dst + 8) = make_uint2(pack_f16(lo[0], lo[1]), pack_f16(lo[2], lo[3]));
       }
     }
     __syncthreads();
@@ -323,15 +350,11 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas
         for (int nt = 0; nt < NT; ++nt) o[i][j][nt][0] = o[i][j][nt][1] = o[i][j][nt][2] = o[i][j][nt][3] = 0.0f;
 
     for (uint32_t i = 0; i < n_mine; ++i) {
-      cp_wait<C::kStages - 2>();
+      const uint32_t page3 = page_of(i + 3);
+      cp_wait<C::kKWait>();
       __syncwarp();
-      {
-        const uint32_t p = page_next;
-        page_next = page_of(i + C::kStages);
-        issue(i + C::kStages - 1, p);
-      }
-      const uint8_t* st = ring + warp * C::kStages * C::kStage + (i % C::kStages) * C::kStage;
-      const float2 sc = *reinterpret_cast<const float2*>(st + 32 * C::kRow);
+      const uint8_t* const ks = k_ring + (i % C::kKSlots) * C::kSlot;
+      const uint8_t* const vs = v_ring + (i % C::kVSlots) * C::kSlot;
       const int pos = (int)((blk0 + warp + i * C::kWarps) * 16);
 
       // scores: keys x rows, four chains
@@ -340,7 +363,7 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s[c][nt][0] = s[c][nt][1] = s[c][nt][2] = s[c][nt][3] = 0.0f;
-      const uint8_t* kp = st + row_k * C::kRow + 16 * t;
+      const uint8_t* kp = ks + row_k * C::kRow + 16 * t;
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
         const uint4 ka = ld16(kp + 64 * c), kb = ld16(kp + 8 * C::kRow + 64 * c);
@@ -364,8 +387,15 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas
         }
       }
 
+      const float k_scale = *reinterpret_cast<const float*>(ks + 16 * C::kRow);
+      __syncwarp();  // every lane has read the keys' slot
+      issue(i + 2, page2, false);
+      cp_wait<C::kVWait>();
+      __syncwarp();
+      const float v_scale = *reinterpret_cast<const float*>(vs + 16 * C::kRow);
+
       // running statistics; the probabilities as the second product's operand
-      const float ev = (float)exp_of(sc.y), inv_v = exp2i(-exp_of(sc.y));
+      const float ev = (float)exp_of(v_scale), inv_v = exp2i(-exp_of(v_scale));
       const bool edge = pos + 15 > pos_min || (a.window && pos <= pos_max - (int)a.window);
       uint32_t p_hi[NT][2], p_lo[NT][2];
 #pragma unroll
@@ -374,7 +404,7 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas
         bool moved = false;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const float cs = sc.x * rs[nt][x];
+          const float cs = k_scale * rs[nt][x];
           tv[0][x] = fmaf(s[0][nt][x] + s[1][nt][x], cs, ev);
           tv[1][x] = fmaf(s[0][nt][2 + x] + s[1][nt][2 + x], cs, ev);
           if (edge) {
@@ -420,7 +450,7 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas
 
       // values: dims x rows.  Thread (g, t) holds the codes of keys t, t + 4,
       // t + 8, t + 12 (the transposed fragments' order) for its dims.
-      const uint8_t* vp = st + (16 + t) * C::kRow + (C::kVec == 16 ? 16 * ((g >> 1) + 4 * (g & 1)) : 8 * g);
+      const uint8_t* vp = vs + t * C::kRow + (C::kVec == 16 ? 16 * ((g >> 1) + 4 * (g & 1)) : 8 * g);
 #pragma unroll
       for (int ps = 0; ps < C::kPasses; ++ps) {
         uint32_t wv[4][C::kVec / 4];
@@ -452,6 +482,10 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas
           }
         }
       }
+      __syncwarp();  // every lane has read the values' slot
+      issue(i + C::kVAhead, C::kVAhead == 2 ? page2 : page1, true);
+      page1 = page2;
+      page2 = page3;
     }
     cp_wait<0>();
     __syncthreads();  // every warp is done with its ring: it now holds the warps' results
@@ -493,8 +527,7 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas
     __syncthreads();
 
     // a unit that lies within this CTA is written; a part of one goes to the workspace
-    const uint32_t u0 = seq0 + unit * w.blocks;
-    const uint32_t c0 = u0 / quota, c1 = (u0 + w.blocks - 1) / quota;
+    const uint32_t c0 = (u0 + C::kStart) / quota, c1 = (u0 + w.cost - 1) / quota;
     const bool whole = c0 == c1;
     constexpr uint32_t kSlot = R * (D + 2);
     auto slot = [&](uint32_t i) {  // part i of this unit: CTA c0 keeps its last part apart from its first
@@ -527,10 +560,16 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas
         my_slot[R * D + 2 * tid] = s_m[0][tid];
         my_slot[R * D + 2 * tid + 1] = s_tot[tid];
       }
-      // merge in groups of kMergeGroup parts, then the groups: the last CTA to
-      // arrive at each reads the parts in their order
-      const uint32_t parts = c1 - c0 + 1, grp = (blockIdx.x - c0) / kMergeGroup;
-      uint32_t stride = 1, n = min(kMergeGroup, parts - grp * kMergeGroup), p0 = grp * kMergeGroup;
+      // merge in groups of parts, then the groups' results: the last CTA to
+      // arrive at each reads the parts in their order.  Groups of about the
+      // square root of the parts keep both levels short.
+      const uint32_t parts = c1 - c0 + 1;
+      uint32_t size = 4;
+      while (size < kMergeGroup && size * size < parts) size += 2;
+      const bool one = parts <= kMergeGroup;
+      if (one) size = kMergeGroup;
+      const uint32_t grp = (blockIdx.x - c0) / size;
+      uint32_t stride = 1, p0 = grp * size, n = min(size, parts - p0);
       uint32_t* counter = a.counters + c0 + p0;
       for (;;) {
         __syncthreads();
@@ -542,30 +581,45 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas
         __syncthreads();
         if (!s_last) break;
         __threadfence();
-        for (uint32_t r = tid; r < n_rows; r += kThreads) {
+        // the parts' statistics, one a thread, while their sums are on the way
+        for (uint32_t i = tid; i < n * R; i += kThreads) {
+          const uint32_t k = i / R, r = i % R;
+          const float2 ml = __ldcg(reinterpret_cast<const float2*>(slot(p0 + k * stride) + R * D + 2 * r));
+          s_f[k][r] = ml.x;
+          s_pl[k][r] = ml.y;
+        }
+        constexpr uint32_t kItems = (R * D / 4 + kThreads - 1) / kThreads, kBatch = 8;
+        float4 y[kBatch];
+        auto fetch = [&](uint32_t i, uint32_t k0) {
+          const uint32_t r = i / (D / 4), d = i % (D / 4) * 4;
+#pragma unroll
+          for (uint32_t k = 0; k < kBatch; ++k)
+            if (k0 + k < n && r < n_rows) y[k] = __ldcg(reinterpret_cast<const float4*>(slot(p0 + (k0 + k) * stride) + r * D + d));
+        };
+        fetch(tid, 0);
+        __syncthreads();
+        if (tid < (uint32_t)R) {
           float top = neg_inf(), sum = 0.0f;
-          for (uint32_t i = 0; i < n; ++i) top = fmaxf(top, __ldcg(slot(p0 + i * stride) + R * D + 2 * r));
-          for (uint32_t i = 0; i < n; ++i) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(slot(p0 + i * stride) + R * D + 2 * r));
-            const float f = part_weight(ml.x, top);
-            s_f[i][r] = f;
-            sum += ml.y * f;
+          for (uint32_t k = 0; k < n; ++k) top = fmaxf(top, s_f[k][tid]);
+          for (uint32_t k = 0; k < n; ++k) {
+            const float f = part_weight(s_f[k][tid], top);
+            s_f[k][tid] = f;
+            sum += s_pl[k][tid] * f;
           }
-          s_m[0][r] = top;
-          s_tot[r] = sum;
+          s_m[0][tid] = top;
+          s_tot[tid] = sum;
         }
         __syncthreads();
-        const bool done = p0 == 0 && (stride > 1 || parts <= kMergeGroup);
-        for (uint32_t i = tid; i < n_rows * (D / 4); i += kThreads) {
-          const uint32_t r = i / (D / 4), d = i % (D / 4) * 4;
+        const bool done = one || stride > 1;
+#pragma unroll 1
+        for (uint32_t it = 0; it < kItems; ++it) {
+          const uint32_t i = tid + it * kThreads, r = i / (D / 4), d = i % (D / 4) * 4;
+          if (r >= n_rows) break;
           float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          for (uint32_t k0 = 0; k0 < n; k0 += 8) {  // 8 loads in flight
-            float4 y[8];
+          for (uint32_t k0 = 0; k0 < n; k0 += kBatch) {
+            if (it + k0 > 0) fetch(i, k0);
 #pragma unroll
-            for (uint32_t k = 0; k < 8; ++k)
-              if (k0 + k < n) y[k] = __ldcg(reinterpret_cast<const float4*>(slot(p0 + (k0 + k) * stride) + r * D + d));
-#pragma unroll
-            for (uint32_t k = 0; k < 8; ++k)
+            for (uint32_t k = 0; k < kBatch; ++k)
               if (k0 + k < n) {
                 const float f = s_f[k0 + k][r];
                 v.x += y[k].x * f, v.y += y[k].y * f, v.z += y[k].z * f, v.w += y[k].w * f;
@@ -583,27 +637,27 @@ __global__ void __launch_bounds__(AttendCfg<D>::kWarps * 32, AttendCfg<D>::kCtas
           slot(p0)[R * D + 2 * tid] = s_m[0][tid];
           slot(p0)[R * D + 2 * tid + 1] = s_tot[tid];
         }
-        n = (parts + kMergeGroup - 1) / kMergeGroup;
-        stride = kMergeGroup;
+        n = (parts + size - 1) / size;
+        stride = size;
         p0 = 0;
         counter = a.counters + kAttendMaxCtas + c0;
       }
     }
-    cur += n_blk;
+    cur = stop;
     __syncthreads();  // shared memory is reused by the next segment
   }
 }
 
 template <int D, int NT, typename T>
 cudaError_t launch(const AttendArgs& a, uint32_t sms, int device, cudaStream_t s) {
-  using C = AttendCfg<D>;
+  using C = AttendCfg<D, NT>;
   // two parts of every CTA fit the workspace
   const size_t slot = 2 * 8 * NT * (D + 2) * sizeof(float);
   uint32_t grid = sms * C::kCtas;
   grid = grid < kAttendMaxCtas ? grid : kAttendMaxCtas;
   grid = grid < a.work_bytes / slot ? grid : (uint32_t)(a.work_bytes / slot);
   constexpr int kSmem = C::kRing + (D / 16) * NT * 32 * (Elem<T>::kExact ? 16 : 8);
-  static_assert(C::kWarps * 8 * NT * D * 4 <= C::kRing, "the warps' results fit the ring");
+  static_assert(C::kWarps * 8 * NT * D * 4 <= kSmem, "the warps' results fit the ring");
   static std::atomic<uint8_t> attr_set[kAttrDevices];
   const cudaError_t e = smem_attr_once(attr_set, device, attend_kernel<D, NT, T>, kSmem);
   if (e != cudaSuccess) return e;
