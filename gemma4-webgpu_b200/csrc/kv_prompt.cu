@@ -63,11 +63,27 @@ __device__ __forceinline__ float ex2p(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+// Two f32 operations an instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return r;
+}
 __device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
 
 // Instruction descriptor, kind::f16: D fp32, A and B f16, A K-major, M = 128;
 // B K-major, or MN-major (its rows in shared memory are the K index).
-__device__ __forceinline__ uint32_t idesc_f16_m128(uint32_t n, bool b_mn) {
+__host__ __device__ constexpr uint32_t idesc_f16_m128(uint32_t n, bool b_mn) {
   return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
@@ -213,81 +229,116 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
       const bool edge = k0 + (int)kPKeys - 1 > tile_first || (a.window && k0 <= tile_last - (int)a.window);
       const int last = row_pos - k0, first = a.window ? last - (int)a.window + 1 : -1;  // columns first..last are seen
 
-      float top = ninf();
+      // this tile's block constants: t = score * cs + ev
+      auto block_cs = [&](uint32_t i) { return fmaxf(__shfl_sync(0xffffffffu, sc, i) * row_c, 1e-37f); };
+      auto block_ev = [&](uint32_t i) { return __shfl_sync(0xffffffffu, sc, 8 + i); };
+      auto mask = [&](float(&v)[32], uint32_t c) {
+        if (edge) {
 #pragma unroll
-      for (uint32_t c = 0; c < 4; ++c) {
-        float v[32];
-        tmem_ld32(s_col + 32 * c, v);
+          for (int i = 0; i < 32; ++i) {
+            const int col = (int)(32 * c) + i;
+            if (col > last || col < first) v[i] = ninf();
+          }
+        }
+      };
+      auto chunk_top = [&](const float(&v)[32], uint32_t c) {  // the largest t of 32 columns
+        float top = ninf();
 #pragma unroll
         for (uint32_t k = 0; k < 2; ++k) {
-          if (edge) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int col = (int)(32 * c + 16 * k) + i;
-              if (col > last || col < first) v[16 * k + i] = ninf();
-            }
-          }
           float bm = v[16 * k];
 #pragma unroll
           for (int i = 1; i < 16; ++i) bm = fmaxf(bm, v[16 * k + i]);
-          const float ks = __shfl_sync(0xffffffffu, sc, 2 * c + k), ev = __shfl_sync(0xffffffffu, sc, 8 + 2 * c + k);
-          top = fmaxf(top, bm == ninf() ? ninf() : fmaf(bm, ks * row_c, ev));
+          top = fmaxf(top, fmaf(bm, block_cs(2 * c + k), block_ev(2 * c + k)));
         }
-      }
-      // move the reference when the new maximum is far above it
-      const bool move = top > m + kLazy || (m == ninf() && top > ninf());
-      if (__any_sync(0xffffffffu, move)) {
-        const float mn = move ? top : m;
-        const float corr = move && m > ninf() ? ex2p(m - mn) : 1.0f;
-        if (j > 0 && __any_sync(0xffffffffu, corr != 1.0f)) {
-          if (!warp_wait(&o_done[group], (j - 1) & 1u, spin)) {
-            failed = true;
-            break;
-          }
-          tc_fence_after();
+        return top;
+      };
+      // move the reference where `top` is far above it; the row's sums follow,
+      // O and the tile's first `c` chunks of P among them
+      auto move = [&](float top, uint32_t c) {
+        const bool up = top > m + kLazy || (m == ninf() && top > ninf());
+        if (!__any_sync(0xffffffffu, up)) return true;
+        const float mn = up ? top : m;
+        const float corr = up && m > ninf() ? ex2p(m - mn) : 1.0f;
+        if (__any_sync(0xffffffffu, corr != 1.0f)) {
+          if (j > 0) {
+            if (!warp_wait(&o_done[group], (j - 1) & 1u, spin)) return false;
+            tc_fence_after();
 #pragma unroll 1
-          for (uint32_t c = 0; c < C::kOut; c += 16) {
+            for (uint32_t i = 0; i < C::kOut; i += 16) {
+              float o[16];
+              tmem_ld16(o_col + i, o);
+              uint32_t w[16];
+#pragma unroll
+              for (int k = 0; k < 16; ++k) w[k] = __float_as_uint(o[k] * corr);
+              tmem_st16(o_col + i, w);
+            }
+          }
+          const __half2 c2 = __float2half2_rn(corr);
+          tmem_wait_st();
+#pragma unroll 1
+          for (uint32_t i = 0; i < c; ++i) {
             float o[16];
-            tmem_ld16(o_col + c, o);
+            tmem_ld16(s_col + 16 * i, o);
             uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(o[i] * corr);
-            tmem_st16(o_col + c, w);
+            for (int k = 0; k < 16; ++k) {
+              const uint32_t bits = __float_as_uint(o[k]);
+              const __half2 p = __hmul2(*reinterpret_cast<const __half2*>(&bits), c2);
+              w[k] = *reinterpret_cast<const uint32_t*>(&p);
+            }
+            tmem_st16(s_col + 16 * i, w);
           }
           tmem_wait_st();
         }
         l *= corr;
         m = mn;
+        return true;
+      };
+
+      float va[32], vb[32];
+      if (__any_sync(0xffffffffu, m == ninf())) {
+        // rows without a reference yet: the tile's largest t first
+        float top = ninf();
+#pragma unroll 1
+        for (uint32_t c = 0; c < 4; ++c) {
+          tmem_ld32(s_col + 32 * c, va);
+          mask(va, c);
+          top = fmaxf(top, chunk_top(va, c));
+        }
+        if (!move(top, 0)) {
+          failed = true;
+          break;
+        }
       }
-      const float ref = m == ninf() ? 0.0f : m - kPromptShift;
+      tmem_ld32_start(s_col, va);
 #pragma unroll
       for (uint32_t c = 0; c < 4; ++c) {
-        float v[32];
-        tmem_ld32(s_col + 32 * c, v);
+        float(&v)[32] = c & 1u ? vb : va;
+        tmem_ld32_wait(v);
+        if (c < 3) tmem_ld32_start(s_col + 32 * (c + 1), c & 1u ? va : vb);
+        mask(v, c);
+        if (!move(chunk_top(v, c), c)) failed = true;
+        const float ref = m == ninf() ? 0.0f : m - kPromptShift;
         uint32_t w[16];
 #pragma unroll
         for (uint32_t k = 0; k < 2; ++k) {
-          const float ks = __shfl_sync(0xffffffffu, sc, 2 * c + k), ev = __shfl_sync(0xffffffffu, sc, 8 + 2 * c + k);
-          const float cs = ks * row_c, off = ev - ref;
-          float sum = 0.0f;
+          const float ev = block_ev(2 * c + k), off = ev - ref, cs = block_cs(2 * c + k);
+          const float2 cs2 = make_float2(cs, cs), off2 = make_float2(off, off);
+          float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            float x = fmaf(v[16 * k + i], cs, off), y = fmaf(v[16 * k + i + 1], cs, off);
-            if (edge) {
-              const int col = (int)(32 * c + 16 * k) + i;
-              if (col > last || col < first) x = ninf();
-              if (col + 1 > last || col + 1 < first) y = ninf();
-            }
-            x = ex2p(x);
-            y = ex2p(y);
-            sum += x + y;
-            const __half2 hh = __floats2half2_rn(x, y);
+            float2 x = fma2(make_float2(v[16 * k + i], v[16 * k + i + 1]), cs2, off2);
+            x.x = ex2p(x.x);
+            x.y = ex2p(x.y);
+            sum = add2(sum, x);
+            const __half2 hh = __floats2half2_rn(x.x, x.y);
             w[8 * k + i / 2] = *reinterpret_cast<const uint32_t*>(&hh);
           }
-          l = fmaf(sum, exp2i(-(int)ev), l);
+          l = fmaf(sum.x + sum.y, exp2i(-(int)ev), l);
         }
         tmem_st16(s_col + 16 * c, w);
       }
+      if (failed) break;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -319,9 +370,25 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
     constexpr uint32_t kRowsIt = 32 / kLanes;     // rows a load instruction of a warp covers
     constexpr uint32_t kIts = 32 / kRowsIt;       // a warp converts 32 of the tile's 128 keys
     const uint32_t cw = warp - 4 * C::kTiles, x = lane % kLanes, rsub = lane / kLanes;
-    uint32_t seq = 0;
     bool meta_bad = false;
-    auto fill = [&](bool is_v, uint32_t j, uint32_t chunk) {
+    // chunk `seq` in the order the MMAs take them: K0; then, per tile j, V_j and
+    // K_{j+1} (two tiles a CTA), or K_{j+1} and V_j
+    constexpr uint32_t kPer = C::kKChunks + C::kVChunks;
+    const uint32_t chunks = n_tiles * kPer;
+    auto load = [&](uint32_t seq, uint4(&code)[kIts]) {
+      bool is_v;
+      uint32_t j, chunk;
+      if (seq < C::kKChunks) {
+        is_v = false, j = 0, chunk = seq;
+      } else {
+        j = (seq - C::kKChunks) / kPer;
+        const uint32_t r = (seq - C::kKChunks) % kPer;
+        const bool v_first = C::kTiles == 2 || j + 1 == n_tiles;
+        const uint32_t lead = v_first ? C::kVChunks : C::kKChunks;
+        is_v = v_first == (r < lead);
+        chunk = r < lead ? r : r - lead;
+        if (!is_v) ++j;
+      }
       const uint32_t pos_w = key0 + j * kPKeys + cw * 32;  // the warp's first key, a multiple of 16
       const uint32_t d0 = (is_v ? half * C::kOut : 0) + chunk * C::kChunk + 16 * x;
       const uint8_t* base[2];
@@ -337,7 +404,6 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
             meta_bad = true;
         }
       }
-      uint4 code[kIts];
 #pragma unroll
       for (uint32_t i = 0; i < kIts; ++i) {
         const uint32_t row = i * kRowsIt + rsub;  // of the warp's 32; block row / 16
@@ -346,6 +412,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
         if (p != nullptr && pos_w + row < s.kv)  // slots past the end are zeros, whatever they hold
           code[i] = __ldg(reinterpret_cast<const uint4*>(p + (row & 15u) * D));
       }
+    };
+    auto convert = [&](uint32_t seq, const uint4(&code)[kIts]) {
       const uint32_t st = seq % C::kRing, use = seq / C::kRing;
       if (use > 0 && !warp_wait(&empty[st], (use - 1) & 1u, spin)) {
         failed = true;
@@ -369,61 +437,76 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[st]);
-      ++seq;
     };
-    // in the order the MMAs take them
-    if (n_tiles) {
-      for (uint32_t c = 0; c < C::kKChunks && !failed; ++c) fill(false, 0, c);
-      for (uint32_t j = 0; j < n_tiles && !failed; ++j) {
-        if (C::kTiles == 2)
-          for (uint32_t c = 0; c < C::kVChunks && !failed; ++c) fill(true, j, c);
-        if (j + 1 < n_tiles)
-          for (uint32_t c = 0; c < C::kKChunks && !failed; ++c) fill(false, j + 1, c);
-        if (C::kTiles == 1)
-          for (uint32_t c = 0; c < C::kVChunks && !failed; ++c) fill(true, j, c);
+    // the next chunk's codes are on their way while this one is converted
+    uint4 ca[kIts], cb[kIts];
+    if (chunks) load(0, ca);
+    for (uint32_t seq = 0; seq < chunks && !failed; seq += 2) {
+      if (seq + 1 < chunks) load(seq + 1, cb);
+      convert(seq, ca);
+      if (seq + 1 < chunks && !failed) {
+        if (seq + 2 < chunks) load(seq + 2, ca);
+        convert(seq + 1, cb);
       }
     }
     if (__any_sync(0xffffffffu, meta_bad) && lane == 0) atomicOr(a.status, kStatusKvMeta);
-  } else if (lane == 0 && n_tiles) {
-    // ---- MMA issue ------------------------------------------------------------------
-    const uint32_t steps = n_tiles * C::kTiles;
-    const uint32_t id_s = idesc_f16_m128(kPKeys, false), id_o = idesc_f16_m128(C::kChunk, true);
-    const uint64_t dq = smem_desc(smem_u32(sq), 1024, 2), dk = smem_desc(smem_u32(ring), 1024, 2);
-    const uint64_t dv = smem_desc(smem_u32(ring), 1024, 2, 16384);  // the same bytes, keys as the K index
-    uint32_t seq = 0, k_seq = 0, v_seq = 0;  // chunks taken; first chunk of the current key and value tiles
+  } else if (n_tiles) {
+    // ---- MMA issue: the warp stays converged and one lane issues, so that
+    // descriptors live in uniform registers (a stream under a divergent branch
+    // with addresses computed per MMA took 135 cycles an MMA instead of 65)
+    const uint32_t steps = __shfl_sync(0xffffffffu, n_tiles * C::kTiles, 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint32_t sq_u = __shfl_sync(0xffffffffu, smem_u32(sq), 0), ring_u = sq_u + C::kTiles * C::kQBytes;
+    const bool leader = elect_lane();
+    constexpr uint32_t id_s = idesc_f16_m128(kPKeys, false), id_o = idesc_f16_m128(C::kChunk, true);
+    uint32_t st = 0, ph = 0;                     // next chunk's ring slot and its phase
+    uint32_t k_st[C::kKChunks], v_st[C::kVChunks];  // slots of the current key and value tiles
+    auto take = [&](uint32_t& slot_of) {         // the next chunk, once it has landed
+      slot_of = st;
+      const bool ok = warp_wait(&full[st], ph, spin);
+      st = st + 1 == C::kRing ? 0 : st + 1;
+      ph ^= st == 0 ? 1u : 0u;
+      return ok;
+    };
     auto scores = [&](uint32_t u) {
-      const uint32_t tile = u % C::kTiles;
-      if (tile == 0) k_seq = seq, seq += C::kKChunks;
-      for (uint32_t c = 0; c < C::kKChunks; ++c) {
-        const uint32_t st = (k_seq + c) % C::kRing;
-        if (tile == 0 && !mbar_wait(&full[st], ((k_seq + c) / C::kRing) & 1u, spin)) return false;
-        tc_fence_after();
+      const uint32_t tile = C::kTiles == 2 ? u & 1u : 0;
 #pragma unroll
-        for (uint32_t kk = 0; kk < C::kChunk / 16; ++kk)
-          umma_f16(tmem + (u & 1u) * 128,
-                      dq + (tile * C::kQBytes + (c * (C::kChunk / 64) + kk / 4) * 16384 + (kk % 4) * 32) / 16,
-                      dk + (st * C::kChunkBytes + (kk / 4) * 16384 + (kk % 4) * 32) / 16, id_s, c + kk > 0);
-        if (tile == C::kTiles - 1) umma_commit(&empty[st]);
+      for (uint32_t c = 0; c < C::kKChunks; ++c) {
+        if (tile == 0 && !take(k_st[c])) return false;
+        tc_fence_after();
+        const uint64_t da = smem_desc(sq_u + tile * C::kQBytes + c * (C::kChunk / 64) * 16384, 1024, 2);
+        const uint64_t db = smem_desc(ring_u + k_st[c] * C::kChunkBytes, 1024, 2);
+        if (leader) {
+#pragma unroll
+          for (uint32_t kk = 0; kk < C::kChunk / 16; ++kk)
+            umma_f16(tm + (u & 1u) * 128, da + ((kk / 4) * 16384 + (kk % 4) * 32) / 16,
+                     db + ((kk / 4) * 16384 + (kk % 4) * 32) / 16, id_s, c + kk > 0);
+          if (tile == C::kTiles - 1) umma_commit(&empty[k_st[c]]);
+          if (c == C::kKChunks - 1) umma_commit(&s_full[u & 1u]);
+        }
+        __syncwarp();
       }
-      umma_commit(&s_full[u & 1u]);
       return true;
     };
     auto values = [&](uint32_t u) {
-      const uint32_t tile = u % C::kTiles, j = u / C::kTiles;
-      if (!mbar_wait(&p_full[u & 1u], (u >> 1) & 1u, spin)) return false;
-      tc_fence_after();
-      if (tile == 0) v_seq = seq, seq += C::kVChunks;
-      for (uint32_t c = 0; c < C::kVChunks; ++c) {
-        const uint32_t st = (v_seq + c) % C::kRing;
-        if (tile == 0 && !mbar_wait(&full[st], ((v_seq + c) / C::kRing) & 1u, spin)) return false;
-        tc_fence_after();
+      const uint32_t tile = C::kTiles == 2 ? u & 1u : 0;
+      if (!warp_wait(&p_full[u & 1u], (u >> 1) & 1u, spin)) return false;
 #pragma unroll
-        for (uint32_t kk = 0; kk < kPKeys / 16; ++kk)
-          umma_f16_ts(tmem + C::kOCol + tile * C::kOut + c * C::kChunk, tmem + (u & 1u) * 128 + kk * 8,
-                          dv + (st * C::kChunkBytes + kk * 2048) / 16, id_o, j > 0 || kk > 0);
-        if (tile == C::kTiles - 1) umma_commit(&empty[st]);
+      for (uint32_t c = 0; c < C::kVChunks; ++c) {
+        if (tile == 0 && !take(v_st[c])) return false;
+        tc_fence_after();
+        // the chunk's bytes with its keys as the K index
+        const uint64_t db = smem_desc(ring_u + v_st[c] * C::kChunkBytes, 1024, 2, 16384);
+        const uint32_t acc = u >= C::kTiles ? 1u : 0u;
+        if (leader) {
+#pragma unroll
+          for (uint32_t kk = 0; kk < kPKeys / 16; ++kk)
+            umma_f16_ts(tm + C::kOCol + tile * C::kOut + c * C::kChunk, tm + (u & 1u) * 128 + kk * 8,
+                        db + kk * 2048 / 16, id_o, kk > 0 ? 1u : acc);
+          if (tile == C::kTiles - 1) umma_commit(&empty[v_st[c]]);
+          if (c == C::kVChunks - 1) umma_commit(&o_done[tile]);
+        }
+        __syncwarp();
       }
-      umma_commit(&o_done[tile]);
       return true;
     };
     bool ok = scores(0);
