@@ -14,8 +14,8 @@
 // shared memory, O += P V with P in tensor memory.  f16 holds every e4m3 code
 // and every f16 or bf16 row (after a power of two per row) exactly; P is
 // rounded once to f16's 11 bits.
-//   warps 0 .. 4 kTiles - 1   softmax, one thread a row: S from tensor memory,
-//                             statistics, P back over S
+//   warps 0 .. 8 kTiles - 1   softmax, two threads a row (64 keys each): S from
+//                             tensor memory, statistics, P back over S
 //   the next 4                read codes through the block table, convert them
 //                             to f16 and store them as swizzled operand chunks
 //                             (128 keys x 128 dims) in a ring
@@ -52,8 +52,9 @@ struct PromptCfg {
   static constexpr uint32_t kKChunks = D / kChunk, kVChunks = kOut / kChunk;
   static constexpr uint32_t kChunkBytes = kPKeys * kChunk * 2;
   static constexpr uint32_t kQBytes = 128 * D * 2;                 // one tile's rows
-  static constexpr uint32_t kRing = D == 512 ? 3 : (D == 64 ? 6 : 5);
-  static constexpr uint32_t kWarps = 4 * kTiles + 5;
+  static constexpr uint32_t kRing = D == 512 ? 3 : (D == 256 ? 5 : 4);
+  static constexpr uint32_t kSoft = 8 * kTiles;                    // softmax warps
+  static constexpr uint32_t kWarps = kSoft + 5;
   static constexpr size_t kSmem = 1024 + kTiles * kQBytes + kRing * kChunkBytes;
   static constexpr uint32_t kOCol = 256;                           // first column of O
 };
@@ -107,6 +108,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
   uint8_t* const sq = smem;                             // [kTiles][D / 64][128 rows][128 bytes], swizzled
   uint8_t* const ring = smem + C::kTiles * C::kQBytes;  // [kRing][kChunk / 64][128 keys][128 bytes], swizzled
   __shared__ uint64_t full[C::kRing], empty[C::kRing], s_full[2], p_full[2], o_done[C::kTiles];
+  __shared__ float s_pair[C::kTiles * 4][2][32];  // what a row's two threads tell each other: 256 bytes a pair of warps
   __shared__ uint32_t s_tmem;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   const uint32_t G = a.group, RT = 128 * C::kTiles;
@@ -142,26 +144,29 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
     }
     for (uint32_t i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[i], 8);
     }
     for (uint32_t i = 0; i < C::kTiles; ++i) mbar_init(&o_done[i], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == C::kWarps - 1) tmem_alloc512(&s_tmem);
 
-  // the rows' operand: f16 under a power of two per row, K-major, 128-byte swizzle
+  // the rows' operand: f16 under a power of two per row, K-major, 128-byte
+  // swizzle; each of a row's two threads takes half of its dims
   float row_c = 0.0f;  // what a score is multiplied with, before the key block's scale
   int row_pos = -1;
-  const uint32_t group = warp / 4, r = tid & 127u;
-  if (warp < 4 * C::kTiles) {
-    const uint32_t rr = row0 + group * 128 + r;
-    const bool live = group * 128 + r < n_rows;
-    const T* src = static_cast<const T*>(a.q) + (uint64_t)(s.t0 + (live ? rr / G : 0)) * a.q_stride +
-                   (h * G + (live ? rr % G : 0)) * D;
+  const uint32_t group = warp / 8, side = (warp >> 2) & 1u, r = tid & 127u;
+  const bool soft = warp < C::kSoft;
+  const uint32_t rr = row0 + group * 128 + r;
+  const bool live = soft && group * 128 + r < n_rows;
+  const T* const src = static_cast<const T*>(a.q) + (uint64_t)(s.t0 + (live ? rr / G : 0)) * a.q_stride +
+                       (h * G + (live ? rr % G : 0)) * D + side * (D / 2);
+  if (soft) {
     float mx = 0.0f;
     if (live) {
       row_pos = pos0 + (int)(rr / G);
-      for (uint32_t d = 0; d < (uint32_t)D; d += 8) {
+#pragma unroll 4
+      for (uint32_t d = 0; d < (uint32_t)D / 2; d += 8) {
         float x[8];
         load_elems(src + d, x);
 #pragma unroll
@@ -169,14 +174,21 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
           if (fabsf(x[i]) <= 3.402823466e38f) mx = fmaxf(mx, fabsf(x[i]));
       }
     }
+    s_pair[group * 4 + (warp & 3u)][side][lane] = mx;
+  }
+  __syncthreads();
+  if (soft) {
+    const float mx = fmaxf(s_pair[group * 4 + (warp & 3u)][0][lane], s_pair[group * 4 + (warp & 3u)][1][lane]);
     int e = 13 - ((int)(__float_as_uint(mx) >> 23) - 127);
     e = mx == 0.0f ? 0 : min(max(e, -110), 110);
     const float up = a.scale_log2 < 0.0f ? -exp2i(e) : exp2i(e);
     row_c = fabsf(a.scale_log2) * exp2i(-e);
     uint8_t* const dst = sq + group * C::kQBytes + r * 128;
-    for (uint32_t d = 0; d < (uint32_t)D; d += 8) {
+#pragma unroll 4
+    for (uint32_t d0 = 0; d0 < (uint32_t)D / 2; d0 += 8) {
+      const uint32_t d = side * (D / 2) + d0;
       float x[8] = {};
-      if (live) load_elems(src + d, x);
+      if (live) load_elems(src + d0, x);
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -194,44 +206,42 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
   const uint32_t tmem = s_tmem;
   bool failed = false;
 
-  if (warp < 4 * C::kTiles) {
-    // ---- softmax: this thread's row --------------------------------------------
+  if (soft) {
+    // ---- softmax: this thread's half of a row --------------------------------------
     const uint32_t lane_off = (32u * (warp & 3u)) << 16;
     const uint32_t o_col = tmem + lane_off + C::kOCol + group * C::kOut;
     const int tile_first = pos0 + (int)((row0 + group * 128) / G);  // the positions of this tile's rows
     const int tile_last = pos0 + (int)(min(row0 + group * 128 + 127, rows - 1) / G);
-    // lane l < 8: the key scale of the tile's block l; l < 16: the value scale of block l - 8
+    const uint32_t pair_bar = 1 + group * 4 + (warp & 3u);  // the two warps of these rows
+    float* const mine = s_pair[group * 4 + (warp & 3u)][0];          // theirs alone
+    auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory"); };
+    // lane l < 4: the key scale of block l of this half's 64 keys; l < 8: the value scale's exponent of block l - 4
     auto scale_of = [&](uint32_t j) {
-      const uint32_t pos = key0 + j * kPKeys + 16 * (lane & 7u);
+      const uint32_t pos = key0 + j * kPKeys + 64 * side + 16 * (lane & 3u);
       float v = 1.0f;
-      if (lane < 16 && pos < s.kv) {
+      if (lane < 8 && pos < s.kv) {
         uint64_t blk;
-        if (kv_block(a.c, table[pos >> a.c.page_shift], h, pos, &blk)) v = (lane < 8 ? a.c.ks : a.c.vs)[blk];
+        if (kv_block(a.c, table[pos >> a.c.page_shift], h, pos, &blk)) v = (lane < 4 ? a.c.ks : a.c.vs)[blk];
       }
-      return lane < 8 ? v : (float)exp_of(v);
+      return lane < 4 ? v : (float)exp_of(v);
     };
-    float m = ninf(), l = 0.0f;
+    float m = ninf(), l = 0.0f;  // l: of this half's keys
     float sc_next = n_tiles ? scale_of(0) : 0.0f;
     for (uint32_t j = 0; j < n_tiles; ++j) {
       const uint32_t u = C::kTiles == 2 ? 2 * j + group : j, sl = u & 1u;
-      const uint32_t s_col = tmem + lane_off + sl * 128;
+      const uint32_t s_col = tmem + lane_off + sl * 128 + side * 64;  // this half's scores, then its probabilities
       const float sc = sc_next;
       if (j + 1 < n_tiles) sc_next = scale_of(j + 1);
-      // S of step u was issued after the product of step u - 2, and commits
-      // arrive in their order: o_done is then at most one phase behind j, so
-      // that its parity tells the phase of tile j - 1 below
-      if (!warp_wait(&s_full[sl], (u >> 1) & 1u, spin)) {
-        failed = true;
-        break;
-      }
+      // (a failed wait ends the waiting, not the loop: the other warp of the
+      // pair counts on this one's barriers)
+      if (!failed && !warp_wait(&s_full[sl], (u >> 1) & 1u, spin)) failed = true;
       tc_fence_after();
-      const int k0 = (int)(key0 + j * kPKeys);
+      const int k0 = (int)(key0 + j * kPKeys), h0 = k0 + 64 * (int)side;
       const bool edge = k0 + (int)kPKeys - 1 > tile_first || (a.window && k0 <= tile_last - (int)a.window);
-      const int last = row_pos - k0, first = a.window ? last - (int)a.window + 1 : -1;  // columns first..last are seen
-
-      // this tile's block constants: t = score * cs + ev
+      const int last = row_pos - h0, first = a.window ? last - (int)a.window + 1 : -1;  // columns first..last are seen
+      // a block's constants: t = score * cs + ev
       auto block_cs = [&](uint32_t i) { return fmaxf(__shfl_sync(0xffffffffu, sc, i) * row_c, 1e-37f); };
-      auto block_ev = [&](uint32_t i) { return __shfl_sync(0xffffffffu, sc, 8 + i); };
+      auto block_ev = [&](uint32_t i) { return __shfl_sync(0xffffffffu, sc, 4 + i); };
       auto mask = [&](float(&v)[32], uint32_t c) {
         if (edge) {
 #pragma unroll
@@ -241,84 +251,53 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
           }
         }
       };
-      auto chunk_top = [&](const float(&v)[32], uint32_t c) {  // the largest t of 32 columns
-        float top = ninf();
+      float v[32], top = ninf();
+#pragma unroll
+      for (uint32_t c = 0; c < 2; ++c) {
+        tmem_ld32(s_col + 32 * c, v);
+        mask(v, c);
 #pragma unroll
         for (uint32_t k = 0; k < 2; ++k) {
-          float bm = v[16 * k];
+          float b0 = v[16 * k], b1 = v[16 * k + 1];
 #pragma unroll
-          for (int i = 1; i < 16; ++i) bm = fmaxf(bm, v[16 * k + i]);
-          top = fmaxf(top, fmaf(bm, block_cs(2 * c + k), block_ev(2 * c + k)));
+          for (int i = 2; i < 16; i += 2) {
+            b0 = fmaxf(b0, v[16 * k + i]);
+            b1 = fmaxf(b1, v[16 * k + i + 1]);
+          }
+          top = fmaxf(top, fmaf(fmaxf(b0, b1), block_cs(2 * c + k), block_ev(2 * c + k)));
         }
-        return top;
-      };
-      // move the reference where `top` is far above it; the row's sums follow,
-      // O and the tile's first `c` chunks of P among them
-      auto move = [&](float top, uint32_t c) {
-        const bool up = top > m + kLazy || (m == ninf() && top > ninf());
-        if (!__any_sync(0xffffffffu, up)) return true;
+      }
+      // both threads of a row go by the same rounded value; two buffers, by tile parity
+      __nv_bfloat16* const told = reinterpret_cast<__nv_bfloat16*>(mine) + (j & 1u) * 64;
+      told[side * 32 + lane] = __float2bfloat16_rn(top);
+      pair_sync();
+      top = fmaxf(__bfloat162float(told[lane]), __bfloat162float(told[32 + lane]));
+      // move the reference when the largest t is far above it; the row's sums follow
+      const bool up = top > m + kLazy || (m == ninf() && top > ninf());
+      if (__any_sync(0xffffffffu, up)) {
         const float mn = up ? top : m;
         const float corr = up && m > ninf() ? ex2p(m - mn) : 1.0f;
-        if (__any_sync(0xffffffffu, corr != 1.0f)) {
-          if (j > 0) {
-            if (!warp_wait(&o_done[group], (j - 1) & 1u, spin)) return false;
-            tc_fence_after();
+        if (j > 0 && __any_sync(0xffffffffu, corr != 1.0f)) {
+          if (!failed && !warp_wait(&o_done[group], (j - 1) & 1u, spin)) failed = true;
+          tc_fence_after();
 #pragma unroll 1
-            for (uint32_t i = 0; i < C::kOut; i += 16) {
-              float o[16];
-              tmem_ld16(o_col + i, o);
-              uint32_t w[16];
-#pragma unroll
-              for (int k = 0; k < 16; ++k) w[k] = __float_as_uint(o[k] * corr);
-              tmem_st16(o_col + i, w);
-            }
-          }
-          const __half2 c2 = __float2half2_rn(corr);
-          tmem_wait_st();
-#pragma unroll 1
-          for (uint32_t i = 0; i < c; ++i) {
+          for (uint32_t c = side * (C::kOut / 2); c < (side + 1) * (C::kOut / 2); c += 16) {
             float o[16];
-            tmem_ld16(s_col + 16 * i, o);
+            tmem_ld16(o_col + c, o);
             uint32_t w[16];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const uint32_t bits = __float_as_uint(o[k]);
-              const __half2 p = __hmul2(*reinterpret_cast<const __half2*>(&bits), c2);
-              w[k] = *reinterpret_cast<const uint32_t*>(&p);
-            }
-            tmem_st16(s_col + 16 * i, w);
+            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(o[i] * corr);
+            tmem_st16(o_col + c, w);
           }
-          tmem_wait_st();
         }
         l *= corr;
         m = mn;
-        return true;
-      };
-
-      float va[32], vb[32];
-      if (__any_sync(0xffffffffu, m == ninf())) {
-        // rows without a reference yet: the tile's largest t first
-        float top = ninf();
-#pragma unroll 1
-        for (uint32_t c = 0; c < 4; ++c) {
-          tmem_ld32(s_col + 32 * c, va);
-          mask(va, c);
-          top = fmaxf(top, chunk_top(va, c));
-        }
-        if (!move(top, 0)) {
-          failed = true;
-          break;
-        }
       }
-      tmem_ld32_start(s_col, va);
+      const float ref = m == ninf() ? 0.0f : m - kPromptShift;
 #pragma unroll
-      for (uint32_t c = 0; c < 4; ++c) {
-        float(&v)[32] = c & 1u ? vb : va;
-        tmem_ld32_wait(v);
-        if (c < 3) tmem_ld32_start(s_col + 32 * (c + 1), c & 1u ? va : vb);
+      for (uint32_t c = 0; c < 2; ++c) {
+        tmem_ld32(s_col + 32 * c, v);
         mask(v, c);
-        if (!move(chunk_top(v, c), c)) failed = true;
-        const float ref = m == ninf() ? 0.0f : m - kPromptShift;
         uint32_t w[16];
 #pragma unroll
         for (uint32_t k = 0; k < 2; ++k) {
@@ -336,23 +315,28 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
           }
           l = fmaf(sum.x + sum.y, exp2i(-(int)ev), l);
         }
-        tmem_st16(s_col + 16 * c, w);
+        tmem_st16(s_col + 16 * c, w);  // over scores that have been read
       }
-      if (failed) break;
       tmem_wait_st();
+      // every tile waits for the product before it, long done by now as a rule:
+      // o_done is then never more than one phase ahead of or behind a wait,
+      // whose parity could not tell two phases apart
+      if (j > 0 && !failed && !warp_wait(&o_done[group], (j - 1) & 1u, spin)) failed = true;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[sl]);
     }
-    // ---- the row's output ---------------------------------------------------------
+    // ---- the row's output, half of its columns a thread -----------------------------
     if (!failed && n_tiles && !warp_wait(&o_done[group], (n_tiles - 1) & 1u, spin)) failed = true;
     tc_fence_after();
-    const bool live = group * 128 + r < n_rows;
+    pair_sync();  // the last tile's maxima have been read
+    mine[side * 32 + lane] = l;
+    pair_sync();
+    l = mine[lane] + mine[32 + lane];
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // nothing seen: zero; NaN stays
-    const uint32_t rr = row0 + group * 128 + r;
     T* const dst = static_cast<T*>(a.out) + (uint64_t)(s.t0 + (live ? rr / G : 0)) * a.out_stride +
                    (h * G + (live ? rr % G : 0)) * D + half * C::kOut;
-    for (uint32_t c = 0; c < C::kOut; c += 16) {
+    for (uint32_t c = side * (C::kOut / 2); c < (side + 1) * (C::kOut / 2); c += 16) {
       float o[16];
       if (n_tiles && !failed) {
         tmem_ld16(o_col + c, o);
@@ -364,65 +348,65 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
       for (int i = 0; i < 16; ++i) o[i] = l != 0.0f ? o[i] * inv : 0.0f;
       if (live) store_elems(dst + c, o);
     }
-  } else if (warp < 4 * C::kTiles + 4) {
+  } else if (warp < C::kSoft + 4) {
     // ---- codes -> f16 operand chunks --------------------------------------------------
-    constexpr uint32_t kLanes = C::kChunk / 16;   // lanes of a row's 16-byte pieces
-    constexpr uint32_t kRowsIt = 32 / kLanes;     // rows a load instruction of a warp covers
-    constexpr uint32_t kIts = 32 / kRowsIt;       // a warp converts 32 of the tile's 128 keys
-    const uint32_t cw = warp - 4 * C::kTiles, x = lane % kLanes, rsub = lane / kLanes;
+    // A warp converts 32 of a chunk's 128 keys in two halves, one 16-token block
+    // each; the next half's codes are on their way while one is converted.
+    constexpr uint32_t kLanes = C::kChunk / 16;  // lanes of a row's 16-byte pieces
+    constexpr uint32_t kRowsIt = 32 / kLanes;    // rows a load instruction of a warp covers
+    constexpr uint32_t kIts = 16 / kRowsIt;
+    const uint32_t cw = warp - C::kSoft, x = lane % kLanes, rsub = lane / kLanes;
     bool meta_bad = false;
-    // chunk `seq` in the order the MMAs take them: K0; then, per tile j, V_j and
-    // K_{j+1} (two tiles a CTA), or K_{j+1} and V_j
-    constexpr uint32_t kPer = C::kKChunks + C::kVChunks;
-    const uint32_t chunks = n_tiles * kPer;
-    auto load = [&](uint32_t seq, uint4(&code)[kIts]) {
-      bool is_v;
-      uint32_t j, chunk;
-      if (seq < C::kKChunks) {
-        is_v = false, j = 0, chunk = seq;
+    // The halves in the order the MMAs take the chunks: K_0; then, per tile j,
+    // V_j and K_{j+1} (two tiles a CTA), or K_{j+1} and V_j.
+    struct Place {
+      uint32_t v, j, c, hf;
+    };
+    auto advance = [&](Place& q) {
+      q.hf ^= 1u;
+      if (q.hf) return;
+      if (++q.c < (q.v ? C::kVChunks : C::kKChunks)) return;
+      q.c = 0;
+      if (C::kTiles == 2) {
+        if (q.v) ++q.j;  // V_j, K_{j+1}
+        q.v ^= 1u;
+      } else if (q.v) {
+        q.j += 2;  // V_j, K_{j+2}
+        q.v = q.j >= n_tiles;
+        if (q.v) q.j = n_tiles - 1;  // no such keys: the last tile's values are next (or the end)
+      } else if (q.j == 0 && n_tiles > 1) {
+        q.j = 1;  // K_0, K_1
       } else {
-        j = (seq - C::kKChunks) / kPer;
-        const uint32_t r = (seq - C::kKChunks) % kPer;
-        const bool v_first = C::kTiles == 2 || j + 1 == n_tiles;
-        const uint32_t lead = v_first ? C::kVChunks : C::kKChunks;
-        is_v = v_first == (r < lead);
-        chunk = r < lead ? r : r - lead;
-        if (!is_v) ++j;
-      }
-      const uint32_t pos_w = key0 + j * kPKeys + cw * 32;  // the warp's first key, a multiple of 16
-      const uint32_t d0 = (is_v ? half * C::kOut : 0) + chunk * C::kChunk + 16 * x;
-      const uint8_t* base[2];
-#pragma unroll
-      for (uint32_t k = 0; k < 2; ++k) {
-        const uint32_t pos = pos_w + 16 * k;
-        base[k] = nullptr;
-        if (pos < s.kv) {
-          uint64_t blk;
-          if (kv_block(a.c, table[pos >> a.c.page_shift], h, pos, &blk))
-            base[k] = (is_v ? a.c.v : a.c.k) + blk * (16 * D) + d0;
-          else
-            meta_bad = true;
-        }
-      }
-#pragma unroll
-      for (uint32_t i = 0; i < kIts; ++i) {
-        const uint32_t row = i * kRowsIt + rsub;  // of the warp's 32; block row / 16
-        code[i] = make_uint4(0, 0, 0, 0);
-        const uint8_t* p = base[i * kRowsIt / 16];
-        if (p != nullptr && pos_w + row < s.kv)  // slots past the end are zeros, whatever they hold
-          code[i] = __ldg(reinterpret_cast<const uint4*>(p + (row & 15u) * D));
+        q.v = 1;  // K_{j+1}, V_j; a single tile: K_0, V_0
+        q.j -= q.j > 0;
       }
     };
-    auto convert = [&](uint32_t seq, const uint4(&code)[kIts]) {
-      const uint32_t st = seq % C::kRing, use = seq / C::kRing;
-      if (use > 0 && !warp_wait(&empty[st], (use - 1) & 1u, spin)) {
-        failed = true;
-        return;
-      }
-      uint8_t* const dst = ring + st * C::kChunkBytes + (x / 4) * 16384;
+    const uint32_t halves = 2 * n_tiles * (C::kKChunks + C::kVChunks);
+    auto page_of = [&](const Place& q) {
+      const uint32_t pos = key0 + q.j * kPKeys + cw * 32 + 16 * q.hf;
+      return pos < s.kv ? table[pos >> a.c.page_shift] : 0xffffffffu;
+    };
+    auto load = [&](const Place& q, uint32_t page, uint4(&code)[kIts]) {
+      const uint32_t pos = key0 + q.j * kPKeys + cw * 32 + 16 * q.hf;
+      uint64_t blk;
+      const bool ok = kv_block(a.c, page, h, pos, &blk);
+      meta_bad |= !ok && pos < s.kv;
+      const uint8_t* const p = (q.v ? a.c.v : a.c.k) + blk * (16 * D) +
+                               ((q.v ? half * C::kOut : 0) + q.c * C::kChunk + 16 * x + rsub * D);
 #pragma unroll
       for (uint32_t i = 0; i < kIts; ++i) {
-        const uint32_t row = cw * 32 + i * kRowsIt + rsub;
+        code[i] = make_uint4(0, 0, 0, 0);
+        if (ok && pos + i * kRowsIt + rsub < s.kv)  // slots past the end are zeros, whatever they hold
+          code[i] = __ldg(reinterpret_cast<const uint4*>(p + i * (kRowsIt * D)));
+      }
+    };
+    uint32_t st = 0, ph = 1;  // ring slot, and the parity of its release before this use
+    auto convert = [&](uint32_t hf, const uint4(&code)[kIts]) {
+      if (hf == 0 && !failed && !warp_wait(&empty[st], ph, spin)) failed = true;  // (the first use passes)
+      uint8_t* const dst = ring + st * C::kChunkBytes + (x / 4) * 16384 + (cw * 32 + hf * 16 + rsub) * 128;
+#pragma unroll
+      for (uint32_t i = 0; i < kIts; ++i) {
+        const uint32_t row7 = (i * kRowsIt + rsub) & 7u;  // the key's row within its swizzle group
         const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
         uint4 o[2];
 #pragma unroll
@@ -431,22 +415,35 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
                             e4m3_to_f16x2(w[2 * k + 1] & 0xffffu), e4m3_to_f16x2(w[2 * k + 1] >> 16));
         // lanes of the second 64 dims store their pieces in the other order: no bank conflict with the first's
         const uint32_t c = 2 * (x & 3u), f = (x >> 2) & 1u;
-        *reinterpret_cast<uint4*>(dst + row * 128 + (((c + f) ^ (row & 7u)) << 4)) = f ? o[1] : o[0];
-        *reinterpret_cast<uint4*>(dst + row * 128 + (((c + 1 - f) ^ (row & 7u)) << 4)) = f ? o[0] : o[1];
+        *reinterpret_cast<uint4*>(dst + i * (kRowsIt * 128) + (((c + f) ^ row7) << 4)) = f ? o[1] : o[0];
+        *reinterpret_cast<uint4*>(dst + i * (kRowsIt * 128) + (((c + 1 - f) ^ row7) << 4)) = f ? o[0] : o[1];
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&full[st]);
+      if (hf) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[st]);
+        st = st + 1 == C::kRing ? 0 : st + 1;
+        ph ^= st == 0 ? 1u : 0u;
+      }
     };
-    // the next chunk's codes are on their way while this one is converted
-    uint4 ca[kIts], cb[kIts];
-    if (chunks) load(0, ca);
-    for (uint32_t seq = 0; seq < chunks && !failed; seq += 2) {
-      if (seq + 1 < chunks) load(seq + 1, cb);
-      convert(seq, ca);
-      if (seq + 1 < chunks && !failed) {
-        if (seq + 2 < chunks) load(seq + 2, ca);
-        convert(seq + 1, cb);
+    if (halves) {
+      Place q{0, 0, 0, 0};
+      uint4 ca[kIts], cb[kIts];
+      load(q, page_of(q), ca);
+      advance(q);
+      uint32_t page = page_of(q);
+#pragma unroll 1
+      for (uint32_t i = 0; i < halves && !failed; i += 2) {
+        load(q, page, cb);  // the second half of this chunk
+        advance(q);
+        page = page_of(q);
+        convert(0, ca);
+        if (i + 2 < halves) {
+          load(q, page, ca);
+          advance(q);
+          page = page_of(q);
+        }
+        convert(1, cb);
       }
     }
     if (__any_sync(0xffffffffu, meta_bad) && lane == 0) atomicOr(a.status, kStatusKvMeta);
@@ -500,7 +497,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
         if (leader) {
 #pragma unroll
           for (uint32_t kk = 0; kk < kPKeys / 16; ++kk)
-            umma_f16_ts(tm + C::kOCol + tile * C::kOut + c * C::kChunk, tm + (u & 1u) * 128 + kk * 8,
+            // P of keys 0..63 lies at the slot's column 0, of 64..127 at its column 64
+            umma_f16_ts(tm + C::kOCol + tile * C::kOut + c * C::kChunk, tm + (u & 1u) * 128 + (kk / 4) * 64 + (kk % 4) * 8,
                         db + kk * 2048 / 16, id_o, kk > 0 ? 1u : acc);
           if (tile == C::kTiles - 1) umma_commit(&empty[v_st[c]]);
           if (c == C::kVChunks - 1) umma_commit(&o_done[tile]);
