@@ -4,8 +4,9 @@
 //
 // Mathematics as in kv_attend.cu: t_j = s_j + e_j (base-2 score plus the value
 // block's exponent), p_j = 2^(t_j - m), O = sum p_j code_j, l = sum p_j 2^-e_j.
-// The reference m of a row moves only when t exceeds it by 8 (p then stays
-// below 2^8, and f16 holds p * 2^7), so the accumulators are rarely rescaled.
+// The reference m of a row moves only when the P of 64 keys, stored times 2^7,
+// add up to more than 2^15 (so no p overflows f16): the sum is needed anyway, a
+// maximum is then not, and the accumulators are rarely rescaled.
 //
 // Work.  A CTA takes 128 * kTiles rows of one sequence and key head (rows:
 // token-major, the query heads of the key head within, so the heads share
@@ -14,12 +15,13 @@
 // shared memory, O += P V with P in tensor memory.  f16 holds every e4m3 code
 // and every f16 or bf16 row (after a power of two per row) exactly; P is
 // rounded once to f16's 11 bits.
-//   warps 0 .. 8 kTiles - 1   softmax, two threads a row (64 keys each): S from
-//                             tensor memory, statistics, P back over S
+//   the first 8               softmax, one thread a row (two tiles) or two (one
+//                             tile, 64 keys each): S from tensor memory,
+//                             statistics, P back over S
 //   the next 4                read codes through the block table, convert them
 //                             to f16 and store them as swizzled operand chunks
 //                             (128 keys x 128 dims) in a ring
-//   the last                  one thread issues the MMAs
+//   the last                  one lane issues the MMAs
 // Tensor memory: two score slots of 128 columns (one per tile, or the two
 // halves of a double buffer when kTiles = 1) and O.  While one slot's softmax
 // runs, the tensor cores work for the other.  Head dims up to 128 run two
@@ -41,7 +43,7 @@ namespace {
 
 constexpr uint32_t kPKeys = 128;        // keys of a tile
 constexpr float kPromptShift = 7.0f;    // P is stored times 2^7
-constexpr float kLazy = 8.0f;           // how far t may exceed the reference
+constexpr float kMostSum = 32768.0f;    // most that 64 keys' P may add up to under a reference (f16 ends at 65504)
 
 template <int D>
 struct PromptCfg {
@@ -53,7 +55,8 @@ struct PromptCfg {
   static constexpr uint32_t kChunkBytes = kPKeys * kChunk * 2;
   static constexpr uint32_t kQBytes = 128 * D * 2;                 // one tile's rows
   static constexpr uint32_t kRing = D == 512 ? 3 : (D == 256 ? 5 : 4);
-  static constexpr uint32_t kSoft = 8 * kTiles;                    // softmax warps
+  static constexpr uint32_t kSplit = 2 / kTiles;                   // softmax threads a row
+  static constexpr uint32_t kSoft = 8;                             // softmax warps
   static constexpr uint32_t kWarps = kSoft + 5;
   static constexpr size_t kSmem = 1024 + kTiles * kQBytes + kRing * kChunkBytes;
   static constexpr uint32_t kOCol = 256;                           // first column of O
@@ -108,7 +111,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
   uint8_t* const sq = smem;                             // [kTiles][D / 64][128 rows][128 bytes], swizzled
   uint8_t* const ring = smem + C::kTiles * C::kQBytes;  // [kRing][kChunk / 64][128 keys][128 bytes], swizzled
   __shared__ uint64_t full[C::kRing], empty[C::kRing], s_full[2], p_full[2], o_done[C::kTiles];
-  __shared__ float s_pair[C::kTiles * 4][2][32];  // what a row's two threads tell each other: 256 bytes a pair of warps
+  __shared__ float s_pair[4][2][32];  // what a row's two threads tell each other: 256 bytes a pair of warps
   __shared__ uint32_t s_tmem;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   const uint32_t G = a.group, RT = 128 * C::kTiles;
@@ -144,7 +147,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
     }
     for (uint32_t i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 8);
+      mbar_init(&p_full[i], 4 * C::kSplit);
     }
     for (uint32_t i = 0; i < C::kTiles; ++i) mbar_init(&o_done[i], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -152,21 +155,22 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
   if (warp == C::kWarps - 1) tmem_alloc512(&s_tmem);
 
   // the rows' operand: f16 under a power of two per row, K-major, 128-byte
-  // swizzle; each of a row's two threads takes half of its dims
+  // swizzle; where a row has two threads each takes half of its dims
   float row_c = 0.0f;  // what a score is multiplied with, before the key block's scale
   int row_pos = -1;
-  const uint32_t group = warp / 8, side = (warp >> 2) & 1u, r = tid & 127u;
+  const uint32_t group = C::kTiles == 2 ? warp >> 2 : 0, side = C::kSplit == 2 ? (warp >> 2) & 1u : 0, r = tid & 127u;
+  constexpr uint32_t kDims = D / C::kSplit;
   const bool soft = warp < C::kSoft;
   const uint32_t rr = row0 + group * 128 + r;
   const bool live = soft && group * 128 + r < n_rows;
   const T* const src = static_cast<const T*>(a.q) + (uint64_t)(s.t0 + (live ? rr / G : 0)) * a.q_stride +
-                       (h * G + (live ? rr % G : 0)) * D + side * (D / 2);
+                       (h * G + (live ? rr % G : 0)) * D + side * kDims;
+  float mx = 0.0f;
   if (soft) {
-    float mx = 0.0f;
     if (live) {
       row_pos = pos0 + (int)(rr / G);
 #pragma unroll 4
-      for (uint32_t d = 0; d < (uint32_t)D / 2; d += 8) {
+      for (uint32_t d = 0; d < kDims; d += 8) {
         float x[8];
         load_elems(src + d, x);
 #pragma unroll
@@ -174,19 +178,19 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
           if (fabsf(x[i]) <= 3.402823466e38f) mx = fmaxf(mx, fabsf(x[i]));
       }
     }
-    s_pair[group * 4 + (warp & 3u)][side][lane] = mx;
+    if (C::kSplit == 2) s_pair[warp & 3u][side][lane] = mx;
   }
-  __syncthreads();
+  if (C::kSplit == 2) __syncthreads();
   if (soft) {
-    const float mx = fmaxf(s_pair[group * 4 + (warp & 3u)][0][lane], s_pair[group * 4 + (warp & 3u)][1][lane]);
+    if (C::kSplit == 2) mx = fmaxf(s_pair[warp & 3u][0][lane], s_pair[warp & 3u][1][lane]);
     int e = 13 - ((int)(__float_as_uint(mx) >> 23) - 127);
     e = mx == 0.0f ? 0 : min(max(e, -110), 110);
     const float up = a.scale_log2 < 0.0f ? -exp2i(e) : exp2i(e);
     row_c = fabsf(a.scale_log2) * exp2i(-e);
     uint8_t* const dst = sq + group * C::kQBytes + r * 128;
 #pragma unroll 4
-    for (uint32_t d0 = 0; d0 < (uint32_t)D / 2; d0 += 8) {
-      const uint32_t d = side * (D / 2) + d0;
+    for (uint32_t d0 = 0; d0 < kDims; d0 += 8) {
+      const uint32_t d = side * kDims + d0;
       float x[8] = {};
       if (live) load_elems(src + d0, x);
       uint32_t w[4];
@@ -207,115 +211,164 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
   bool failed = false;
 
   if (soft) {
-    // ---- softmax: this thread's half of a row --------------------------------------
+    // ---- softmax: this thread's row, or its half of one ------------------------------
+    constexpr uint32_t kBlocks = 8 / C::kSplit;   // 16-key blocks of a tile that the thread has
+    constexpr uint32_t kParts = kBlocks / 4;      // it takes them 64 keys at a time
+    constexpr uint32_t kCols = C::kOut / C::kSplit;  // its columns of O
     const uint32_t lane_off = (32u * (warp & 3u)) << 16;
-    const uint32_t o_col = tmem + lane_off + C::kOCol + group * C::kOut;
+    const uint32_t o_col = tmem + lane_off + C::kOCol + group * C::kOut + side * kCols;
     const int tile_first = pos0 + (int)((row0 + group * 128) / G);  // the positions of this tile's rows
     const int tile_last = pos0 + (int)(min(row0 + group * 128 + 127, rows - 1) / G);
-    const uint32_t pair_bar = 1 + group * 4 + (warp & 3u);  // the two warps of these rows
-    float* const mine = s_pair[group * 4 + (warp & 3u)][0];          // theirs alone
+    const uint32_t pair_bar = 1 + (warp & 3u);        // the two warps of the same rows
+    float* const mine = s_pair[warp & 3u][0];         // theirs alone
     auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory"); };
-    // lane l < 4: the key scale of block l of this half's 64 keys; l < 8: the value scale's exponent of block l - 4
-    auto scale_of = [&](uint32_t j) {
-      const uint32_t pos = key0 + j * kPKeys + 64 * side + 16 * (lane & 3u);
-      float v = 1.0f;
-      if (lane < 8 && pos < s.kv) {
-        uint64_t blk;
-        if (kv_block(a.c, table[pos >> a.c.page_shift], h, pos, &blk)) v = (lane < 4 ? a.c.ks : a.c.vs)[blk];
-      }
-      return lane < 4 ? v : (float)exp_of(v);
+    // whether any row of this warp (and of the one that shares its rows) says so
+    auto any_row = [&](bool x) {
+      if (C::kSplit == 1) return __any_sync(0xffffffffu, x) != 0;
+      uint32_t r;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.or.pred p, %2, 64, q;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(r)
+          : "r"((uint32_t)x), "r"(pair_bar)
+          : "memory");
+      return r != 0;
     };
-    float m = ninf(), l = 0.0f;  // l: of this half's keys
+    // lane i: the key scale of the thread's block i of tile j; lane kBlocks + i: its value scale's exponent
+    auto scale_of = [&](uint32_t j) {
+      const uint32_t pos = key0 + j * kPKeys + 64 * side + 16 * (lane % kBlocks);
+      float v = 1.0f;
+      if (lane < 2 * kBlocks && pos < s.kv) {
+        uint64_t blk;
+        if (kv_block(a.c, table[pos >> a.c.page_shift], h, pos, &blk)) v = (lane < kBlocks ? a.c.ks : a.c.vs)[blk];
+      }
+      return lane < kBlocks ? v : (float)exp_of(v);
+    };
+    float m = ninf(), l = 0.0f;  // l: of this thread's keys
     float sc_next = n_tiles ? scale_of(0) : 0.0f;
     for (uint32_t j = 0; j < n_tiles; ++j) {
       const uint32_t u = C::kTiles == 2 ? 2 * j + group : j, sl = u & 1u;
-      const uint32_t s_col = tmem + lane_off + sl * 128 + side * 64;  // this half's scores, then its probabilities
       const float sc = sc_next;
       if (j + 1 < n_tiles) sc_next = scale_of(j + 1);
       // (a failed wait ends the waiting, not the loop: the other warp of the
       // pair counts on this one's barriers)
       if (!failed && !warp_wait(&s_full[sl], (u >> 1) & 1u, spin)) failed = true;
       tc_fence_after();
-      const int k0 = (int)(key0 + j * kPKeys), h0 = k0 + 64 * (int)side;
+      const int k0 = (int)(key0 + j * kPKeys);
       const bool edge = k0 + (int)kPKeys - 1 > tile_first || (a.window && k0 <= tile_last - (int)a.window);
-      const int last = row_pos - h0, first = a.window ? last - (int)a.window + 1 : -1;  // columns first..last are seen
-      // a block's constants: t = score * cs + ev
-      auto block_cs = [&](uint32_t i) { return fmaxf(__shfl_sync(0xffffffffu, sc, i) * row_c, 1e-37f); };
-      auto block_ev = [&](uint32_t i) { return __shfl_sync(0xffffffffu, sc, 4 + i); };
-      auto mask = [&](float(&v)[32], uint32_t c) {
-        if (edge) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int col = (int)(32 * c) + i;
-            if (col > last || col < first) v[i] = ninf();
+      for (uint32_t part = 0; part < kParts; ++part) {
+        const uint32_t half64 = C::kSplit == 2 ? side : part;                // which 64 keys of the tile
+        const uint32_t s_col = tmem + lane_off + sl * 128 + half64 * 64;     // their scores, then probabilities
+        const int last = row_pos - k0 - 64 * (int)half64;                    // columns first..last are seen
+        const int first = a.window ? last - (int)a.window + 1 : -1;
+        // a block's constants: t = score * cs + ev
+        auto block_cs = [&](uint32_t i) { return fmaxf(__shfl_sync(0xffffffffu, sc, 4 * part + i) * row_c, 1e-37f); };
+        auto block_ev = [&](uint32_t i) { return __shfl_sync(0xffffffffu, sc, kBlocks + 4 * part + i); };
+        auto mask = [&](float(&v)[16], uint32_t c) {
+          if (edge) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int col = (int)(16 * c) + i;
+              if (col > last || col < first) v[i] = ninf();
+            }
           }
-        }
-      };
-      float v[32], top = ninf();
+        };
+        // P under the current reference, and its sum; the sum also tells whether
+        // the reference still serves: every p is below 2^15 if the 64 together are
+        uint32_t w[32];
+        float sum, sum_l[4];  // of the 64 keys, of each block's
+        auto probabilities = [&] {
+          const float ref = m == ninf() ? 0.0f : m - kPromptShift;
+          sum = 0.0f;
 #pragma unroll
-      for (uint32_t c = 0; c < 2; ++c) {
-        tmem_ld32(s_col + 32 * c, v);
-        mask(v, c);
+          for (uint32_t c = 0; c < 4; ++c) {  // a block of 16 keys
+            float v[16];
+            tmem_ld16(s_col + 16 * c, v);
+            mask(v, c);
+            const float off = block_ev(c) - ref, cs = block_cs(c);
+            const float2 cs2 = make_float2(cs, cs), off2 = make_float2(off, off);
+            float2 p = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (uint32_t k = 0; k < 2; ++k) {
-          float b0 = v[16 * k], b1 = v[16 * k + 1];
-#pragma unroll
-          for (int i = 2; i < 16; i += 2) {
-            b0 = fmaxf(b0, v[16 * k + i]);
-            b1 = fmaxf(b1, v[16 * k + i + 1]);
+            for (int i = 0; i < 16; i += 2) {
+              float2 x = fma2(make_float2(v[i], v[i + 1]), cs2, off2);
+              x.x = ex2p(x.x);
+              x.y = ex2p(x.y);
+              p = add2(p, x);
+              const __half2 hh = __floats2half2_rn(x.x, x.y);
+              w[8 * c + i / 2] = *reinterpret_cast<const uint32_t*>(&hh);
+            }
+            sum_l[c] = p.x + p.y;
+            sum += sum_l[c];
           }
-          top = fmaxf(top, fmaf(fmaxf(b0, b1), block_cs(2 * c + k), block_ev(2 * c + k)));
+        };
+        bool above = m == ninf();
+        if (!__all_sync(0xffffffffu, above)) {
+          probabilities();
+          above |= sum > kMostSum;
         }
-      }
-      // both threads of a row go by the same rounded value; two buffers, by tile parity
-      __nv_bfloat16* const told = reinterpret_cast<__nv_bfloat16*>(mine) + (j & 1u) * 64;
-      told[side * 32 + lane] = __float2bfloat16_rn(top);
-      pair_sync();
-      top = fmaxf(__bfloat162float(told[lane]), __bfloat162float(told[32 + lane]));
-      // move the reference when the largest t is far above it; the row's sums follow
-      const bool up = top > m + kLazy || (m == ninf() && top > ninf());
-      if (__any_sync(0xffffffffu, up)) {
-        const float mn = up ? top : m;
-        const float corr = up && m > ninf() ? ex2p(m - mn) : 1.0f;
-        if (j > 0 && __any_sync(0xffffffffu, corr != 1.0f)) {
-          if (!failed && !warp_wait(&o_done[group], (j - 1) & 1u, spin)) failed = true;
-          tc_fence_after();
+        if (any_row(above)) {
+          // move the references that the largest t is far above, and the rows' sums with them
+          float top = ninf();
 #pragma unroll 1
-          for (uint32_t c = side * (C::kOut / 2); c < (side + 1) * (C::kOut / 2); c += 16) {
-            float o[16];
-            tmem_ld16(o_col + c, o);
-            uint32_t w[16];
+          for (uint32_t c = 0; c < 4; ++c) {
+            float v[16];
+            tmem_ld16(s_col + 16 * c, v);
+            mask(v, c);
+            float b0 = v[0];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(o[i] * corr);
-            tmem_st16(o_col + c, w);
+            for (int i = 1; i < 16; ++i) b0 = fmaxf(b0, v[i]);
+            top = fmaxf(top, fmaf(b0, block_cs(c), block_ev(c)));
           }
-        }
-        l *= corr;
-        m = mn;
-      }
-      const float ref = m == ninf() ? 0.0f : m - kPromptShift;
-#pragma unroll
-      for (uint32_t c = 0; c < 2; ++c) {
-        tmem_ld32(s_col + 32 * c, v);
-        mask(v, c);
-        uint32_t w[16];
-#pragma unroll
-        for (uint32_t k = 0; k < 2; ++k) {
-          const float ev = block_ev(2 * c + k), off = ev - ref, cs = block_cs(2 * c + k);
-          const float2 cs2 = make_float2(cs, cs), off2 = make_float2(off, off);
-          float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            float2 x = fma2(make_float2(v[16 * k + i], v[16 * k + i + 1]), cs2, off2);
-            x.x = ex2p(x.x);
-            x.y = ex2p(x.y);
-            sum = add2(sum, x);
-            const __half2 hh = __floats2half2_rn(x.x, x.y);
-            w[8 * k + i / 2] = *reinterpret_cast<const uint32_t*>(&hh);
+          if (C::kSplit == 2) {
+            // both threads of a row go by the same rounded value; two buffers, by tile parity
+            __nv_bfloat16* const told = reinterpret_cast<__nv_bfloat16*>(mine) + (j & 1u) * 64;
+            told[side * 32 + lane] = __float2bfloat16_rn(top);
+            pair_sync();
+            top = fmaxf(__bfloat162float(told[lane]), __bfloat162float(told[32 + lane]));
           }
-          l = fmaf(sum.x + sum.y, exp2i(-(int)ev), l);
+          const bool up = top > m + 1.0f || (m == ninf() && top > ninf());
+          const float mn = up ? top : m;
+          const float corr = up && m > ninf() ? ex2p(m - mn) : 1.0f;
+          if (__any_sync(0xffffffffu, corr != 1.0f)) {
+            if (j > 0) {
+              if (!failed && !warp_wait(&o_done[group], (j - 1) & 1u, spin)) failed = true;
+              tc_fence_after();
+#pragma unroll 1
+              for (uint32_t c = 0; c < kCols; c += 16) {
+                float o[16];
+                tmem_ld16(o_col + c, o);
+                uint32_t ow[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) ow[i] = __float_as_uint(o[i] * corr);
+                tmem_st16(o_col + c, ow);
+              }
+            }
+            if (part > 0) {  // the tile's first 64 probabilities are already stored
+              const __half2 c2 = __float2half2_rn(corr);
+              tmem_wait_st();
+#pragma unroll 1
+              for (uint32_t c = 0; c < 32; c += 16) {
+                float o[16];
+                tmem_ld16(s_col - 64 + c, o);
+                uint32_t ow[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const uint32_t bits = __float_as_uint(o[i]);
+                  const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&bits), c2);
+                  ow[i] = *reinterpret_cast<const uint32_t*>(&x);
+                }
+                tmem_st16(s_col - 64 + c, ow);
+              }
+            }
+          }
+          l *= corr;
+          m = mn;
+          probabilities();
         }
-        tmem_st16(s_col + 16 * c, w);  // over scores that have been read
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) l = fmaf(sum_l[i], exp2i(-(int)block_ev(i)), l);
+        tmem_put32(s_col, w);  // over scores that have been read
       }
       tmem_wait_st();
       // every tile waits for the product before it, long done by now as a rule:
@@ -326,17 +379,19 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[sl]);
     }
-    // ---- the row's output, half of its columns a thread -----------------------------
+    // ---- the row's output (half of its columns) ----------------------------------------
     if (!failed && n_tiles && !warp_wait(&o_done[group], (n_tiles - 1) & 1u, spin)) failed = true;
     tc_fence_after();
-    pair_sync();  // the last tile's maxima have been read
-    mine[side * 32 + lane] = l;
-    pair_sync();
-    l = mine[lane] + mine[32 + lane];
+    if (C::kSplit == 2) {
+      pair_sync();  // the last tile's maxima have been read
+      mine[side * 32 + lane] = l;
+      pair_sync();
+      l = mine[lane] + mine[32 + lane];
+    }
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // nothing seen: zero; NaN stays
     T* const dst = static_cast<T*>(a.out) + (uint64_t)(s.t0 + (live ? rr / G : 0)) * a.out_stride +
-                   (h * G + (live ? rr % G : 0)) * D + half * C::kOut;
-    for (uint32_t c = side * (C::kOut / 2); c < (side + 1) * (C::kOut / 2); c += 16) {
+                   (h * G + (live ? rr % G : 0)) * D + half * C::kOut + side * kCols;
+    for (uint32_t c = 0; c < kCols; c += 16) {
       float o[16];
       if (n_tiles && !failed) {
         tmem_ld16(o_col + c, o);
@@ -393,11 +448,16 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
       meta_bad |= !ok && pos < s.kv;
       const uint8_t* const p = (q.v ? a.c.v : a.c.k) + blk * (16 * D) +
                                ((q.v ? half * C::kOut : 0) + q.c * C::kChunk + 16 * x + rsub * D);
+      if (ok && pos + 16 <= s.kv) {
 #pragma unroll
-      for (uint32_t i = 0; i < kIts; ++i) {
-        code[i] = make_uint4(0, 0, 0, 0);
-        if (ok && pos + i * kRowsIt + rsub < s.kv)  // slots past the end are zeros, whatever they hold
-          code[i] = __ldg(reinterpret_cast<const uint4*>(p + i * (kRowsIt * D)));
+        for (uint32_t i = 0; i < kIts; ++i) code[i] = __ldg(reinterpret_cast<const uint4*>(p + i * (kRowsIt * D)));
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < kIts; ++i) {
+          code[i] = make_uint4(0, 0, 0, 0);
+          if (ok && pos + i * kRowsIt + rsub < s.kv)  // slots past the end are zeros, whatever they hold
+            code[i] = __ldg(reinterpret_cast<const uint4*>(p + i * (kRowsIt * D)));
+        }
       }
     };
     uint32_t st = 0, ph = 1;  // ring slot, and the parity of its release before this use
@@ -407,16 +467,15 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
 #pragma unroll
       for (uint32_t i = 0; i < kIts; ++i) {
         const uint32_t row7 = (i * kRowsIt + rsub) & 7u;  // the key's row within its swizzle group
-        const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
-        uint4 o[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          o[k] = make_uint4(e4m3_to_f16x2(w[2 * k] & 0xffffu), e4m3_to_f16x2(w[2 * k] >> 16),
-                            e4m3_to_f16x2(w[2 * k + 1] & 0xffffu), e4m3_to_f16x2(w[2 * k + 1] >> 16));
         // lanes of the second 64 dims store their pieces in the other order: no bank conflict with the first's
         const uint32_t c = 2 * (x & 3u), f = (x >> 2) & 1u;
-        *reinterpret_cast<uint4*>(dst + i * (kRowsIt * 128) + (((c + f) ^ row7) << 4)) = f ? o[1] : o[0];
-        *reinterpret_cast<uint4*>(dst + i * (kRowsIt * 128) + (((c + 1 - f) ^ row7) << 4)) = f ? o[0] : o[1];
+        const uint32_t w[4] = {f ? code[i].z : code[i].x, f ? code[i].w : code[i].y, f ? code[i].x : code[i].z,
+                               f ? code[i].y : code[i].w};
+#pragma unroll
+        for (uint32_t k = 0; k < 2; ++k)
+          *reinterpret_cast<uint4*>(dst + i * (kRowsIt * 128) + (((c + (f ^ k)) ^ row7) << 4)) =
+              make_uint4(e4m3_to_f16x2(w[2 * k] & 0xffffu), e4m3_to_f16x2(w[2 * k] >> 16),
+                         e4m3_to_f16x2(w[2 * k + 1] & 0xffffu), e4m3_to_f16x2(w[2 * k + 1] >> 16));
       }
       if (hf) {
         fence_proxy_async_smem();
