@@ -96,6 +96,11 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, spin)) != 0;
 }
 
+template <bool kValue>
+struct Bool {
+  static constexpr bool value = kValue;
+};
+
 struct PromptArgs {
   AttendArgs a;
   uint32_t spin;
@@ -266,26 +271,27 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
         auto block_cs = [&](uint32_t i) { return fmaxf(__shfl_sync(0xffffffffu, sc, 4 * part + i) * row_c, 1e-37f); };
         auto block_ev = [&](uint32_t i) { return __shfl_sync(0xffffffffu, sc, kBlocks + 4 * part + i); };
         auto mask = [&](float(&v)[16], uint32_t c) {
-          if (edge) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int col = (int)(16 * c) + i;
-              if (col > last || col < first) v[i] = ninf();
-            }
+          for (int i = 0; i < 16; ++i) {
+            const int col = (int)(16 * c) + i;
+            if (col > last || col < first) v[i] = ninf();
           }
         };
         // P under the current reference, and its sum; the sum also tells whether
         // the reference still serves: every p is below 2^15 if the 64 together are
         uint32_t w[32];
         float sum, sum_l[4];  // of the 64 keys, of each block's
-        auto probabilities = [&] {
+        auto probabilities = [&](auto masked) {
           const float ref = m == ninf() ? 0.0f : m - kPromptShift;
           sum = 0.0f;
+          float vv[2][16];
+          tmem_ld16_start(s_col, vv[0]);
 #pragma unroll
-          for (uint32_t c = 0; c < 4; ++c) {  // a block of 16 keys
-            float v[16];
-            tmem_ld16(s_col + 16 * c, v);
-            mask(v, c);
+          for (uint32_t c = 0; c < 4; ++c) {  // a block of 16 keys, the next on its way
+            float(&v)[16] = vv[c & 1u];
+            tmem_ld16_wait(v);
+            if (c < 3) tmem_ld16_start(s_col + 16 * (c + 1), vv[(c + 1) & 1u]);
+            if constexpr (decltype(masked)::value) mask(v, c);
             const float off = block_ev(c) - ref, cs = block_cs(c);
             const float2 cs2 = make_float2(cs, cs), off2 = make_float2(off, off);
             float2 p = make_float2(0.0f, 0.0f);
@@ -304,7 +310,11 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
         };
         bool above = m == ninf();
         if (!__all_sync(0xffffffffu, above)) {
-          probabilities();
+          // (without branches in it, the four blocks' arithmetic overlaps)
+          if (edge)
+            probabilities(Bool<true>{});
+          else
+            probabilities(Bool<false>{});
           above |= sum > kMostSum;
         }
         if (any_row(above)) {
@@ -364,7 +374,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
           }
           l *= corr;
           m = mn;
-          probabilities();
+          probabilities(Bool<true>{});
         }
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) l = fmaf(sum_l[i], exp2i(-(int)block_ev(i)), l);
