@@ -106,6 +106,70 @@ struct PromptArgs {
   uint32_t spin;
 };
 
+// The rows' operand: f16 under a power of two per row (its reciprocal to
+// row_scale), K-major, 128-byte swizzle.  Each softmax warp takes every
+// kSoft-th group of rows, lanes side by side along a row, four groups' loads
+// in flight.
+template <int D, typename T>
+__device__ __forceinline__ void load_rows(const AttendArgs& a, uint32_t t0, uint32_t row0, uint32_t n_rows, uint32_t h,
+                                          uint8_t* sq, float* row_scale, uint32_t warp, uint32_t lane) {
+  using C = PromptCfg<D>;
+  constexpr uint32_t kLanes = D / 8 < 32 ? D / 8 : 32;  // lanes of a row (8 elements each)
+  constexpr uint32_t kSteps = D / (8 * kLanes);         // loads of a row
+  constexpr uint32_t kRows = 32 / kLanes;               // rows of a group
+  constexpr uint32_t kGroups = C::kTiles * 128 / kRows / C::kSoft, kBatch = kSteps > 1 ? 2 : 4;
+  const uint32_t sub = lane / kLanes, x = lane % kLanes, G = a.group;
+  const uint32_t mask = kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1u) << (sub * kLanes);
+#pragma unroll 1
+  for (uint32_t g0 = 0; g0 < kGroups; g0 += kBatch) {
+    uint4 raw[kBatch][kSteps];
+#pragma unroll
+    for (uint32_t g = 0; g < kBatch; ++g) {
+      const uint32_t row = ((g0 + g) * C::kSoft + warp) * kRows + sub, rr = row0 + row;
+#pragma unroll
+      for (uint32_t k = 0; k < kSteps; ++k) {
+        raw[g][k] = make_uint4(0, 0, 0, 0);
+        if (row < n_rows)
+          raw[g][k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (uint64_t)(t0 + rr / G) * a.q_stride +
+                                                           (h * G + rr % G) * D + 8 * (x + kLanes * k)));
+      }
+    }
+#pragma unroll
+    for (uint32_t g = 0; g < kBatch; ++g) {
+      const uint32_t row = ((g0 + g) * C::kSoft + warp) * kRows + sub;
+      float v[kSteps][8], mx = 0.0f;
+#pragma unroll
+      for (uint32_t k = 0; k < kSteps; ++k) {
+        const T* e = reinterpret_cast<const T*>(&raw[g][k]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          v[k][i] = Elem<T>::to(e[i]);
+          if (fabsf(v[k][i]) <= 3.402823466e38f) mx = fmaxf(mx, fabsf(v[k][i]));
+        }
+      }
+      const uint32_t mb = __reduce_max_sync(mask, __float_as_uint(mx));
+      int e = 13 - ((int)(mb >> 23) - 127);
+      e = mb == 0 ? 0 : min(max(e, -110), 110);
+      const float up = a.scale_log2 < 0.0f ? -exp2i(e) : exp2i(e);
+      if (x == 0) row_scale[row] = exp2i(-e);
+      uint8_t* const dst = sq + (row / 128) * C::kQBytes + (row % 128) * 128;
+#pragma unroll
+      for (uint32_t k = 0; k < kSteps; ++k) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const __half2 hh = __floats2half2_rn(v[k][2 * i] * up, v[k][2 * i + 1] * up);
+          w[i] = *reinterpret_cast<const uint32_t*>(&hh);
+        }
+        const uint32_t d = 8 * (x + kLanes * k);
+        *reinterpret_cast<uint4*>(dst + (d / 64) * 16384 + ((((d % 64) / 8) ^ (row & 7u)) << 4)) =
+            make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+  fence_proxy_async_smem();
+}
+
 template <int D, typename T>
 __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(const PromptArgs pa) {
   using C = PromptCfg<D>;
@@ -117,6 +181,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
   uint8_t* const ring = smem + C::kTiles * C::kQBytes;  // [kRing][kChunk / 64][128 keys][128 bytes], swizzled
   __shared__ uint64_t full[C::kRing], empty[C::kRing], s_full[2], p_full[2], o_done[C::kTiles];
   __shared__ float s_pair[4][2][32];  // what a row's two threads tell each other: 256 bytes a pair of warps
+  __shared__ float s_row[C::kTiles * 128];  // rows' scales
   __shared__ uint32_t s_tmem;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   const uint32_t G = a.group, RT = 128 * C::kTiles;
@@ -159,60 +224,20 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
   }
   if (warp == C::kWarps - 1) tmem_alloc512(&s_tmem);
 
-  // the rows' operand: f16 under a power of two per row, K-major, 128-byte
-  // swizzle; where a row has two threads each takes half of its dims
-  float row_c = 0.0f;  // what a score is multiplied with, before the key block's scale
-  int row_pos = -1;
-  const uint32_t group = C::kTiles == 2 ? warp >> 2 : 0, side = C::kSplit == 2 ? (warp >> 2) & 1u : 0, r = tid & 127u;
-  constexpr uint32_t kDims = D / C::kSplit;
   const bool soft = warp < C::kSoft;
-  const uint32_t rr = row0 + group * 128 + r;
+  const uint32_t group = C::kTiles == 2 ? warp >> 2 : 0, side = C::kSplit == 2 ? (warp >> 2) & 1u : 0, r = tid & 127u;
+  const uint32_t rr = row0 + group * 128 + r;  // a softmax thread's row
   const bool live = soft && group * 128 + r < n_rows;
-  const T* const src = static_cast<const T*>(a.q) + (uint64_t)(s.t0 + (live ? rr / G : 0)) * a.q_stride +
-                       (h * G + (live ? rr % G : 0)) * D + side * kDims;
-  float mx = 0.0f;
-  if (soft) {
-    if (live) {
-      row_pos = pos0 + (int)(rr / G);
-#pragma unroll 4
-      for (uint32_t d = 0; d < kDims; d += 8) {
-        float x[8];
-        load_elems(src + d, x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (fabsf(x[i]) <= 3.402823466e38f) mx = fmaxf(mx, fabsf(x[i]));
-      }
-    }
-    if (C::kSplit == 2) s_pair[warp & 3u][side][lane] = mx;
-  }
-  if (C::kSplit == 2) __syncthreads();
-  if (soft) {
-    if (C::kSplit == 2) mx = fmaxf(s_pair[warp & 3u][0][lane], s_pair[warp & 3u][1][lane]);
-    int e = 13 - ((int)(__float_as_uint(mx) >> 23) - 127);
-    e = mx == 0.0f ? 0 : min(max(e, -110), 110);
-    const float up = a.scale_log2 < 0.0f ? -exp2i(e) : exp2i(e);
-    row_c = fabsf(a.scale_log2) * exp2i(-e);
-    uint8_t* const dst = sq + group * C::kQBytes + r * 128;
-#pragma unroll 4
-    for (uint32_t d0 = 0; d0 < kDims; d0 += 8) {
-      const uint32_t d = side * kDims + d0;
-      float x[8] = {};
-      if (live) load_elems(src + d0, x);
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const __half2 hh = __floats2half2_rn(x[2 * i] * up, x[2 * i + 1] * up);
-        w[i] = *reinterpret_cast<const uint32_t*>(&hh);
-      }
-      *reinterpret_cast<uint4*>(dst + (d / 64) * 16384 + ((((d % 64) / 8) ^ (r & 7u)) << 4)) =
-          make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    fence_proxy_async_smem();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = s_tmem;
+  if (soft) load_rows<D, T>(a, s.t0, row0, n_rows, h, sq, s_row, warp, lane);
+  // every role meets the others once its own start is made: barriers, tensor
+  // memory and the rows are then ready
+  auto start = [&] {
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    return s_tmem;
+  };
+  uint32_t tmem = 0;
   bool failed = false;
 
   if (soft) {
@@ -220,6 +245,10 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
     constexpr uint32_t kBlocks = 8 / C::kSplit;   // 16-key blocks of a tile that the thread has
     constexpr uint32_t kParts = kBlocks / 4;      // it takes them 64 keys at a time
     constexpr uint32_t kCols = C::kOut / C::kSplit;  // its columns of O
+    tmem = start();
+    // what a score is multiplied with, before the key block's scale
+    const float row_c = fabsf(a.scale_log2) * s_row[group * 128 + r];
+    const int row_pos = live ? pos0 + (int)(rr / G) : -1;
     const uint32_t lane_off = (32u * (warp & 3u)) << 16;
     const uint32_t o_col = tmem + lane_off + C::kOCol + group * C::kOut + side * kCols;
     const int tile_first = pos0 + (int)((row0 + group * 128) / G);  // the positions of this tile's rows
@@ -399,8 +428,9 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
       l = mine[lane] + mine[32 + lane];
     }
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // nothing seen: zero; NaN stays
-    T* const dst = static_cast<T*>(a.out) + (uint64_t)(s.t0 + (live ? rr / G : 0)) * a.out_stride +
-                   (h * G + (live ? rr % G : 0)) * D + half * C::kOut + side * kCols;
+    // into the rows' place (every product has read them), 16-byte pieces
+    // permuted by row, then to memory with lanes side by side along a row
+    uint8_t* const stage = sq + group * (128 * C::kOut * 2);
     for (uint32_t c = 0; c < kCols; c += 16) {
       float o[16];
       if (n_tiles && !failed) {
@@ -411,7 +441,23 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[i] = l != 0.0f ? o[i] * inv : 0.0f;
-      if (live) store_elems(dst + c, o);
+#pragma unroll
+      for (uint32_t k = 0; k < 2; ++k) {
+        const float half8[8] = {o[8 * k],     o[8 * k + 1], o[8 * k + 2], o[8 * k + 3],
+                                o[8 * k + 4], o[8 * k + 5], o[8 * k + 6], o[8 * k + 7]};
+        store_elems(reinterpret_cast<T*>(stage + r * (C::kOut * 2) + (((side * kCols + c) / 8 + k) ^ (r & 7u)) * 16), half8);
+      }
+    }
+    asm volatile("bar.sync 5, 256;" ::: "memory");  // the softmax warps
+    constexpr uint32_t kPieces = C::kOut / 8;
+    for (uint32_t i = tid; i < C::kTiles * 128 * kPieces; i += 256) {
+      const uint32_t row = i / kPieces, x = i % kPieces;
+      if (row < n_rows) {
+        const uint32_t at = row0 + row;
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (uint64_t)(s.t0 + at / G) * a.out_stride + (h * G + at % G) * D +
+                                  half * C::kOut + 8 * x) =
+            *reinterpret_cast<const uint4*>(sq + row * (C::kOut * 2) + (x ^ (row & 7u)) * 16);
+      }
     }
   } else if (warp < C::kSoft + 4) {
     // ---- codes -> f16 operand chunks --------------------------------------------------
@@ -495,31 +541,29 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
         ph ^= st == 0 ? 1u : 0u;
       }
     };
-    if (halves) {
-      Place q{0, 0, 0, 0};
-      uint4 ca[kIts], cb[kIts];
-      load(q, page_of(q), ca);
+    Place q{0, 0, 0, 0};
+    uint4 ca[kIts], cb[kIts];
+    uint32_t page = page_of(q);
+    auto load_next = [&](uint4(&to)[kIts]) {
+      load(q, page, to);
       advance(q);
-      uint32_t page = page_of(q);
+      page = page_of(q);
+    };
+    if (halves) load_next(ca);
+    start();
 #pragma unroll 1
-      for (uint32_t i = 0; i < halves && !failed; i += 2) {
-        load(q, page, cb);  // the second half of this chunk
-        advance(q);
-        page = page_of(q);
-        convert(0, ca);
-        if (i + 2 < halves) {
-          load(q, page, ca);
-          advance(q);
-          page = page_of(q);
-        }
-        convert(1, cb);
-      }
+    for (uint32_t i = 0; i < halves && !failed; i += 2) {
+      load_next(cb);  // the second half of this chunk
+      convert(0, ca);
+      if (i + 2 < halves) load_next(ca);
+      convert(1, cb);
     }
     if (__any_sync(0xffffffffu, meta_bad) && lane == 0) atomicOr(a.status, kStatusKvMeta);
-  } else if (n_tiles) {
+  } else {
     // ---- MMA issue: the warp stays converged and one lane issues, so that
     // descriptors live in uniform registers (a stream under a divergent branch
     // with addresses computed per MMA took 135 cycles an MMA instead of 65)
+    tmem = start();
     const uint32_t steps = __shfl_sync(0xffffffffu, n_tiles * C::kTiles, 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
     const uint32_t sq_u = __shfl_sync(0xffffffffu, smem_u32(sq), 0), ring_u = sq_u + C::kTiles * C::kQBytes;
     const bool leader = elect_lane();
@@ -576,7 +620,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
       }
       return true;
     };
-    bool ok = scores(0);
+    bool ok = steps == 0 || scores(0);
     if (ok && steps > 1) ok = scores(1);
     for (uint32_t u = 0; u < steps && ok; ++u) {
       ok = values(u);
