@@ -99,14 +99,31 @@ __device__ __forceinline__ float finite(float x, bool* bad) {
 template <typename T>
 __global__ void __launch_bounds__(512) append_kernel(const AppendArgs a) {
   const uint32_t D = a.c.dim, H = a.c.heads, per = D / 16;
+  // the block's sequence: the last one that starts at or before this slot.  Its
+  // thread has loaded the values along, so one round of loads tells all.
+  __shared__ KvSeq s_seq;
+  __shared__ uint32_t s_first;
   uint32_t b = 0;
   for (uint32_t i0 = 0; i0 < a.b.seqs; i0 += blockDim.x) {
     const uint32_t i = i0 + threadIdx.x;
-    b += __syncthreads_count(i < a.b.seqs && a.b.q_start[i] / 16 + 2 * i <= blockIdx.x);
+    uint32_t first = 0xffffffffu;
+    KvSeq mine{};
+    if (i < a.b.seqs) {
+      mine = kv_seq(a.b, a.c.page_shift, i);
+      first = a.b.q_start[i] / 16 + 2 * i;
+    }
+    const uint32_t n = __syncthreads_count(first <= blockIdx.x);
+    if (n && threadIdx.x == n - 1) {
+      s_seq = mine;
+      s_first = first;
+    }
+    b += n;
+    if (n < blockDim.x) break;
   }
+  __syncthreads();
   if (b == 0) return;
   --b;
-  const KvSeq s = kv_seq(a.b, a.c.page_shift, b);
+  const KvSeq s = s_seq;
   if (s.bad) {
     if (threadIdx.x == 0) atomicOr(a.status, kStatusKvMeta);
     return;
@@ -115,7 +132,7 @@ __global__ void __launch_bounds__(512) append_kernel(const AppendArgs a) {
   // new tokens whose position would be negative (n > kv_len) are left out
   const uint32_t skip = s.n > s.kv ? s.n - s.kv : 0;
   const uint32_t p0 = s.kv - (s.n - skip);
-  const uint32_t bs = (p0 / 16 + blockIdx.x - (a.b.q_start[b] / 16 + 2 * b)) * 16;  // the block's first position
+  const uint32_t bs = (p0 / 16 + blockIdx.x - s_first) * 16;  // the block's first position
   const bool range_bad = skip > 0 || (a.rot && s.kv > a.rope_len);
   if (range_bad && threadIdx.x == 0) atomicOr(a.status, kStatusKvMeta);
   if (bs >= s.kv) return;

@@ -588,15 +588,19 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kWarps * 32, AttendCfg<D, NT
           s_f[k][r] = ml.x;
           s_pl[k][r] = ml.y;
         }
-        constexpr uint32_t kItems = (R * D / 4 + kThreads - 1) / kThreads, kBatch = 8;
-        float4 y[kBatch];
-        auto fetch = [&](uint32_t i, uint32_t k0) {
-          const uint32_t r = i / (D / 4), d = i % (D / 4) * 4;
+        // a thread's pieces of the sums, kBatch parts at a time: as many loads in flight as registers allow
+        constexpr uint32_t kFlight = C::kCtas == 2 ? 8 : 16, kItems = (R * D / 4 + kThreads - 1) / kThreads;
+        constexpr uint32_t kBatch = kItems < kFlight ? kFlight / kItems : 1;
+        const bool has = tid < R * D / 4;  // (head dim 64 has fewer pieces than threads)
+        float4 y[kItems][kBatch], v[kItems];
+        auto fetch = [&](uint32_t k0) {
 #pragma unroll
           for (uint32_t k = 0; k < kBatch; ++k)
-            if (k0 + k < n && r < n_rows) y[k] = __ldcg(reinterpret_cast<const float4*>(slot(p0 + (k0 + k) * stride) + r * D + d));
+#pragma unroll
+            for (uint32_t it = 0; it < kItems; ++it)
+              if (has && k0 + k < n) y[it][k] = __ldcg(reinterpret_cast<const float4*>(slot(p0 + (k0 + k) * stride)) + tid + it * kThreads);
         };
-        fetch(tid, 0);
+        fetch(0);
         __syncthreads();
         if (tid < (uint32_t)R) {
           float top = neg_inf(), sum = 0.0f;
@@ -610,26 +614,30 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kWarps * 32, AttendCfg<D, NT
           s_tot[tid] = sum;
         }
         __syncthreads();
+#pragma unroll
+        for (uint32_t it = 0; it < kItems; ++it) v[it] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t k0 = 0; k0 < n; k0 += kBatch) {
+          if (k0) fetch(k0);
+#pragma unroll
+          for (uint32_t k = 0; k < kBatch; ++k)
+            if (has && k0 + k < n) {
+#pragma unroll
+              for (uint32_t it = 0; it < kItems; ++it) {
+                const float f = s_f[k0 + k][(tid + it * kThreads) / (D / 4)];
+                v[it].x += y[it][k].x * f, v[it].y += y[it][k].y * f, v[it].z += y[it][k].z * f, v[it].w += y[it][k].w * f;
+              }
+            }
+        }
         const bool done = one || stride > 1;
-#pragma unroll 1
+#pragma unroll
         for (uint32_t it = 0; it < kItems; ++it) {
           const uint32_t i = tid + it * kThreads, r = i / (D / 4), d = i % (D / 4) * 4;
-          if (r >= n_rows) break;
-          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          for (uint32_t k0 = 0; k0 < n; k0 += kBatch) {
-            if (it + k0 > 0) fetch(i, k0);
-#pragma unroll
-            for (uint32_t k = 0; k < kBatch; ++k)
-              if (k0 + k < n) {
-                const float f = s_f[k0 + k][r];
-                v.x += y[k].x * f, v.y += y[k].y * f, v.z += y[k].z * f, v.w += y[k].w * f;
-              }
-          }
+          if (r >= n_rows) continue;
           if (done) {
             const float tot = s_tot[r], inv = tot != 0.0f ? 1.0f / tot : 0.0f;
-            put(r, d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+            put(r, d, make_float4(v[it].x * inv, v[it].y * inv, v[it].z * inv, v[it].w * inv));
           } else {
-            *reinterpret_cast<float4*>(slot(p0) + r * D + d) = v;  // each element read by this thread alone before
+            *reinterpret_cast<float4*>(slot(p0) + r * D + d) = v[it];  // each piece read by this thread alone before
           }
         }
         if (done) break;

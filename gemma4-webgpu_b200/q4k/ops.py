@@ -107,7 +107,7 @@ class KVCache:
                 raise ValueError(f"{name} must be [pages, kv_heads, page_size / {KV_BLOCK}]")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, page, dim
-        self.device = k.device
+        self.device, self.index = k.device, k.get_device()
         self._struct = _KVCacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, page,
                                       heads, dim)
         self._addr = ctypes.addressof(self._struct)
@@ -144,6 +144,7 @@ class Context:
         if rc != _lib.Q4K_OK:
             raise Q4KError(rc, f"q4k_create(device={self.device.index}) failed")
         self._h = handle.value
+        self._index = self.device.index
         self._args = bytearray(256)  # the argument record of the call being made
         self._args_addr = ctypes.addressof((ctypes.c_char * 256).from_buffer(self._args))
 
@@ -440,32 +441,39 @@ class Context:
     def _current_stream(self, stream: torch.cuda.Stream | None) -> int:
         if stream is not None:
             return stream.cuda_stream
-        return torch._C._cuda_getCurrentRawStream(self.device.index)  # no Stream object for the common call
+        return torch._C._cuda_getCurrentRawStream(self._index)  # no Stream object for the common call
 
     def _rows(self, t: torch.Tensor, name: str, dtype: torch.dtype, tokens: int, dim: int) -> tuple[int, int]:
         """(heads, row stride) of rows [tokens, heads, head_dim]: any row stride, heads side by side."""
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor")
-        if t.get_device() != self.device.index:
-            raise ValueError(f"{name} is on {t.device}, expected {self.device}")
         if t.dtype is not dtype:
             raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
-        shape = t.shape
-        if len(shape) != 3 or shape[0] != tokens or shape[2] != dim:
+        if t.get_device() != self._index:
+            raise ValueError(f"{name} is on {t.device}, expected {self.device}")
+        try:
+            n, heads, width = t.shape
+            row, head, one = t.stride()
+        except ValueError:
+            n = -1
+        if n != tokens or width != dim:
             raise ValueError(f"{name} must be [{tokens}, heads, {dim}]")
-        row, head, one = t.stride()
-        heads = shape[1]
         if one != 1 or (head != dim and heads > 1):
             raise ValueError(f"{name}: the heads of a row must be contiguous")
         return heads, row if tokens > 1 else heads * dim
+
+    def _like(self, t: torch.Tensor, other: torch.Tensor) -> bool:
+        """Whether rows `t` are laid out as `other`, which _rows has checked."""
+        return (isinstance(t, torch.Tensor) and t.dtype is other.dtype and t.get_device() == self._index
+                and t.shape == other.shape and t.stride() == other.stride())
 
     def _need_batch(self, cache: KVCache, block_table: torch.Tensor, q_start: torch.Tensor,
                     kv_len: torch.Tensor) -> tuple[int, int]:
         """(sequences, block table columns)."""
         if not isinstance(cache, KVCache):
             raise TypeError("cache must be a KVCache")
-        index = self.device.index
-        if cache.k.get_device() != index:
+        index = self._index
+        if cache.index != index:
             raise ValueError(f"cache is on {cache.k.device}, expected {self.device}")
         for t, name in ((block_table, "block_table"), (q_start, "q_start"), (kv_len, "kv_len")):
             if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == index
@@ -495,12 +503,14 @@ class Context:
         if code is None:
             raise TypeError(f"k has dtype {dtype}, expected one of {tuple(DTYPES)}")
         heads, k_stride = self._rows(k, "k", dtype, tokens, dim)
-        v_heads, v_stride = self._rows(v, "v", dtype, tokens, dim)
+        v_heads, v_stride = (heads, k_stride) if self._like(v, k) else self._rows(v, "v", dtype, tokens, dim)
         if heads != cache.kv_heads or v_heads != heads:
             raise ValueError(f"k and v must have the cache's {cache.kv_heads} heads")
         rope_len = rope_dim = rope_ptr = q_heads = q_stride = qo_stride = q_ptr = qo_ptr = 0
         if rope is not None:
-            _need(rope, torch.float32, "rope", self.device)
+            if not (isinstance(rope, torch.Tensor) and rope.dtype is torch.float32 and rope.get_device() == self._index
+                    and rope.is_contiguous()):
+                _need(rope, torch.float32, "rope", self.device)
             shape = rope.shape
             if len(shape) != 3 or shape[2] != 2:
                 raise ValueError("rope must be [positions, pairs, 2]")
@@ -509,7 +519,8 @@ class Context:
             q_heads, q_stride = self._rows(q, "q", dtype, tokens, dim)
             if q_out is None:
                 q_out = torch.empty((tokens, q_heads, dim), dtype=dtype, device=self.device)
-            qo_heads, qo_stride = self._rows(q_out, "q_out", dtype, tokens, dim)
+            qo_heads, qo_stride = (q_heads, q_stride) if self._like(q_out, q) else self._rows(q_out, "q_out", dtype,
+                                                                                             tokens, dim)
             if qo_heads != q_heads:
                 raise ValueError("q_out and q differ in shape")
             q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
@@ -542,7 +553,7 @@ class Context:
             raise ValueError("window and max_q must lie in 0 .. 2^31 - 1")
         if out is None:
             out = torch.empty((tokens, heads, dim), dtype=dtype, device=self.device)
-        out_heads, out_stride = self._rows(out, "out", dtype, tokens, dim)
+        out_heads, out_stride = (heads, q_stride) if self._like(out, q) else self._rows(out, "out", dtype, tokens, dim)
         if out_heads != heads:
             raise ValueError("out and q differ in shape")
         _ATTENTION.pack_into(self._args, 0, block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), seqs, tokens,
@@ -568,7 +579,7 @@ class Context:
         entropy [rows], top_logprob [rows, top], top_token int32 [rows, top])."""
         if not isinstance(logits, torch.Tensor):
             raise TypeError("logits must be a torch.Tensor")
-        if logits.get_device() != self.device.index:
+        if logits.get_device() != self._index:
             raise ValueError(f"logits is on {logits.device}, expected {self.device}")
         code = DTYPES.get(logits.dtype)
         if code is None:
@@ -579,7 +590,9 @@ class Context:
         row, one = logits.stride()
         if one != 1 and V > 1:
             raise ValueError("logits must be [rows, V] with contiguous rows")
-        _need(tokens, torch.int32, "tokens", self.device)
+        if not (isinstance(tokens, torch.Tensor) and tokens.dtype is torch.int32 and tokens.get_device() == self._index
+                and tokens.is_contiguous()):
+            _need(tokens, torch.int32, "tokens", self.device)
         if tokens.numel() != rows:
             raise ValueError("tokens must hold one id for each row")
         if not 0 <= top <= min(32, V):
