@@ -1,0 +1,102 @@
+"""Decoding with a paged 8-bit cache: the attention block and the answer of a
+serving step, put together from the framework's calls.
+
+The reference runs q/k/v, the rotation, the cache stores, the three attention
+passes and the o product per layer and token (src/engine.ts:1547-1586), then
+the LM head and its sampling (:1686-1741).  CachedDecoder does the same for a
+batch of sequences of any lengths, prompts and single tokens alike:
+
+    q, k, v  = Wq x, Wk x, Wv x                    Context.gemv (Q4_K)
+    append k, v; rotate q, k by position           Context.kv_append
+    a        = attention over the cache            Context.paged_attention
+    x        = x + Wo a                            Context.gemv
+    ...                                            every layer, its own cache
+    logits   = W_head x                            Context.gemv
+    log probabilities, entropy, alternatives       Context.token_logprobs
+
+Norms and the FFN, which lie between these in the model, are not run, as in
+the other synthetic steps of this package.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import synth
+from .decode import E2BShape, layer_shapes, matrix_seed, LMHEAD_SEED
+from .ops import Context, KVCache
+
+
+def rope_table(positions: int, dim: int, theta: float = 10000.0, device: torch.device | str = "cpu") -> torch.Tensor:
+    """(cos, sin) of every position and pair, f32 [positions, dim / 2, 2], from f64 angles
+    (the reference's frequencies, shaders/rope.wgsl:12)."""
+    freq = theta ** (-torch.arange(0, dim, 2, dtype=torch.float64, device=device) / dim)
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.stack([angle.cos(), angle.sin()], -1).float()
+
+
+@dataclass
+class Answer:
+    """What a step returns for each of its rows."""
+
+    logprob: torch.Tensor  # f32 [rows]: of the row's given token (NaN: none given)
+    entropy: torch.Tensor  # f32 [rows]
+    top_logprob: torch.Tensor  # f32 [rows, top]
+    top_token: torch.Tensor  # int32 [rows, top]
+
+
+class CachedDecoder:
+    """Q4_K attention blocks over a paged 8-bit cache, and the LM head's
+    answer, for up to `seqs` sequences of up to `positions` tokens."""
+
+    def __init__(self, ctx: Context, shape: E2BShape | None = None, layers: int = 2, seqs: int = 4,
+                 positions: int = 2048, page_size: int = 64, window: int = 0, vocab: int | None = None):
+        self.ctx, self.shape = ctx, shape or E2BShape()
+        s, dev = self.shape, ctx.device
+        self.vocab, self.window, self.page_size = vocab or s.vocab, window, page_size
+        self.head_dim = s.kv  # one key head, as E2B
+        self.q_heads = s.q // s.kv
+        mats = layer_shapes(s)
+        up = lambda m, n, seed: torch.from_numpy(synth.q4k_matrix(m, n, seed)).to(dev)  # noqa: E731
+        self.weights = [{n: up(*mats[n], matrix_seed(i, n)) for n in ("q", "k", "v", "o")} for i in range(layers)]
+        self.head = up(self.vocab, s.hidden, LMHEAD_SEED)
+        self.rope = rope_table(positions, self.head_dim, device=dev)
+        columns = -(-positions // page_size)
+        self.caches = [KVCache.allocate(seqs * columns, 1, page_size, self.head_dim, dev) for _ in range(layers)]
+        # every sequence owns its columns' pages; a server would hand them out as it goes
+        self.block_table = torch.arange(seqs * columns, dtype=torch.int32, device=dev).view(seqs, columns)
+        self.lengths = [0] * seqs
+        self.positions = positions
+
+    def _matmul(self, w: torch.Tensor, x: torch.Tensor, m: int, n: int) -> torch.Tensor:
+        return self.ctx.gemv(w, x, m, n)
+
+    def step(self, x: torch.Tensor, counts: list[int], tokens: torch.Tensor | None = None, top: int = 0) -> Answer:
+        """Runs counts[b] new rows of each sequence b (x: f32 [sum(counts),
+        hidden], sequence by sequence) and answers for every row; tokens: the
+        id whose log probability each row is asked for."""
+        s, ctx, dev = self.shape, self.ctx, self.ctx.device
+        rows = sum(counts)
+        if len(counts) != len(self.lengths) or x.shape != (rows, s.hidden):
+            raise ValueError(f"counts must have {len(self.lengths)} entries and x be [sum(counts), {s.hidden}]")
+        if any(n + c > self.positions for n, c in zip(self.lengths, counts)):
+            raise ValueError(f"a sequence would exceed {self.positions} positions")
+        self.lengths = [n + c for n, c in zip(self.lengths, counts)]
+        starts = [0]
+        for c in counts:
+            starts.append(starts[-1] + c)
+        i32 = dict(dtype=torch.int32, device=dev)
+        q_start, kv_len = torch.tensor(starts, **i32), torch.tensor(self.lengths, **i32)
+        batch = (self.block_table, q_start, kv_len)
+        for w, cache in zip(self.weights, self.caches):
+            q = self._matmul(w["q"], x, s.q, s.hidden).view(rows, self.q_heads, self.head_dim)
+            k = self._matmul(w["k"], x, s.kv, s.hidden).view(rows, 1, self.head_dim)
+            v = self._matmul(w["v"], x, s.kv, s.hidden).view(rows, 1, self.head_dim)
+            ctx.kv_append(cache, k, v, self.rope, *batch, q=q, q_out=q)
+            a = ctx.paged_attention(cache, q, *batch, max(counts), self.head_dim**-0.5, window=self.window)
+            x = x + self._matmul(w["o"], a.view(rows, s.q), s.hidden, s.q)
+        logits = self._matmul(self.head, x, self.vocab, s.hidden)
+        if tokens is None:
+            tokens = torch.full((rows,), -1, **i32)
+        return Answer(*ctx.token_logprobs(logits, tokens, top=top, cap=s.softcap))

@@ -1,0 +1,108 @@
+"""CPU checks of the cached-attention calls: the packed argument records match
+the C structs, null arguments are rejected before any CUDA call, and the plain
+restatement the GPU tests use is itself right."""
+from __future__ import annotations
+
+import ctypes
+import re
+
+import pytest
+import torch
+
+import kv_reference as R
+from conftest import ROOT
+
+HEADER = (ROOT / "include" / "q4k.h").read_text()
+SIZES = {"uint32_t": (4, "I"), "uint64_t": (8, "Q"), "float": (4, "f")}
+
+
+def fields(struct: str) -> list[tuple[str, int, str]]:
+    """(name, size, struct code) of each member of a typedef'd struct of the header."""
+    body = re.search(r"typedef struct \{([^}]*)\} %s;" % struct, HEADER).group(1)
+    out = []
+    for line in re.sub(r"/\*.*?\*/", "", body, flags=re.S).split(";"):
+        m = re.match(r"\s*(?:const )?(\w+)\s*(\*?)\s*(\w+)\s*$", line)
+        if m:
+            out.append((m.group(3), *((8, "Q") if m.group(2) else SIZES[m.group(1)])))
+    return out
+
+
+def layout(struct: str) -> tuple[str, int]:
+    """The struct-module format of a C struct with natural alignment, and its size."""
+    fmt, at = "", 0
+    for _, size, code in fields(struct):
+        pad = -at % size
+        fmt += "x" * pad + code
+        at += pad + size
+    pad = -at % 8
+    return fmt + "x" * pad, at + pad
+
+
+@pytest.mark.parametrize("name,struct,after", [
+    ("_KV_BATCH", "q4k_kv_batch", None), ("_KV_APPEND", "q4k_kv_append_args", "q4k_kv_batch"),
+    ("_ATTENTION", "q4k_attention_args", "q4k_kv_batch"), ("_LOGPROBS", "q4k_logprobs_args", None)])
+def test_records_match_the_header(name, struct, after):
+    from q4k import ops
+
+    rec = getattr(ops, name)
+    fmt = (layout(after)[0] if after else "") + layout(struct)[0]
+    assert rec.format.lstrip("<") == fmt
+    assert rec.size == sum(layout(x)[1] for x in (after, struct) if x)
+
+
+def test_cache_struct_matches_the_header():
+    from q4k.ops import _KVCacheStruct
+
+    assert [n for n, _ in _KVCacheStruct._fields_] == [n for n, _, _ in fields("q4k_kv_cache")]
+    assert ctypes.sizeof(_KVCacheStruct) == layout("q4k_kv_cache")[1]
+
+
+def test_null_arguments():
+    import q4k._lib as ql
+
+    L = ql.lib()
+    assert L.q4k_kv_append(None, None, None, None, None) == -1
+    assert L.q4k_paged_attention(None, None, None, None, None) == -1
+    assert L.q4k_token_logprobs(None, None, None) == -1
+
+
+def test_cache_checks_its_tensors():
+    from q4k import KVCache
+
+    k = torch.zeros(2, 1, 16, 64, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    s = torch.ones(2, 1, 1)
+    KVCache(k, k, s, s)
+    assert KVCache(k, k, s, s).bytes_per_token() == 2 * (64 + 0.25)
+    for args, err in [((k.view(torch.uint8), k, s, s), TypeError), ((k, k[:1], s, s), ValueError),
+                      ((k, k, s[:1], s), ValueError), ((k, k, s, s.double()), TypeError), ((k[0], k, s, s), ValueError),
+                      ((k[:, :, :, :32], k, s, s), ValueError)]:
+        with pytest.raises(err):
+            KVCache(*args)
+
+
+def test_reference_scales_and_rotation():
+    amax = torch.tensor([448.0, 448.1, 0.0, 1.0, 1e30, 0.875], dtype=torch.float64)
+    assert R.scale_of(amax).tolist() == [1.0, 2.0, 2.0**-60, 2.0**-8, 2.0**60, 2.0**-9]
+    tab = R.rope_table(8, 64).double()
+    x = torch.randn(8, 1, 64, dtype=torch.float64)
+    y = R.rotate(x, tab[:, None, :, 0], tab[:, None, :, 1])
+    assert torch.allclose(y.norm(dim=-1), x.norm(dim=-1), rtol=1e-6)
+    # scores depend on the distance alone
+    q, k = x[0, 0], x[1, 0]
+    at = lambda v, p: R.rotate(v, tab[p, :, 0], tab[p, :, 1])  # noqa: E731
+    assert torch.allclose(at(q, 5) @ at(k, 3), at(q, 7) @ at(k, 5), atol=1e-4)
+
+
+def test_reference_attention_against_differences():
+    """The restatement's weights are a softmax: raising a key's score moves the output toward its value."""
+    pr = R.Problem([1], [20], 1, 1, 64, 16, seed=3)
+    k, v = R.dequant(pr.k, pr.k_scale), R.dequant(pr.v, pr.v_scale)
+    base = R.attention(pr.q, k, v, pr.table, pr.q_start, pr.kv, 0.125)[0, 0]
+    eps = 1e-5
+    page, slot = int(pr.table[0, 0]), 7
+    moved = k.clone()
+    moved[page, 0, slot] += eps * pr.q[0, 0] / pr.q[0, 0].norm() ** 2 / 0.125  # that score + eps
+    out = R.attention(pr.q, moved, v, pr.table, pr.q_start, pr.kv, 0.125)[0, 0]
+    s = (R.gather(k, pr.table[0], 20)[0] @ pr.q[0, 0]) * 0.125
+    p = torch.softmax(s, 0)[slot]
+    assert torch.allclose((out - base) / eps, p * (v[page, 0, slot] - base), atol=1e-4)
