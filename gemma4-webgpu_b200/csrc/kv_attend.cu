@@ -1,7 +1,7 @@
 // q4k_paged_attention for few rows per sequence (a decode step): attention
 // over the paged 8-bit cache (kv_cache.cuh).  The reference runs three passes
-// over an f32 cache (shaders/attn_score.wgsl:14-39, softmax.wgsl,
-// attn_output.wgsl:10-22); this is one pass with running softmax statistics.
+// over an f32 cache (shaders/attn_score.wgsl, softmax.wgsl,
+// attn_output.wgsl); this is one pass with running softmax statistics.
 //
 // Mathematics.  With s_j the base-2 logits of a row and 2^e_j the value scale
 // of key j's block, let t_j = s_j + e_j and m the running maximum of t.  Then
@@ -28,6 +28,15 @@
 // probabilities, so that f32 results hold f32 accuracy.  For f16 and bf16
 // rows the probabilities are rounded once to f16's 11 bits: less than the
 // output's own rounding.
+//
+// Measured on B200 (8 rows unless said; the cache read once would take):
+//   2 x 131072 tokens, head dim 256, bf16     34 us (20.5): reading ends at
+//     26 us, joining 74 parts a unit in two levels takes the rest
+//   128 x <= 4001 tokens, 8 heads of 128, 4 rows, bf16   100 us (72): the
+//     instruction latency of 16 warps an SM
+//   33 x <= 8193 tokens, head dim 512, f32    40 us (19): the hi + lo products
+//   2048 tokens, head dim 256, f32            11 us: metadata, page, copy and
+//     merge, one after the other
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -49,7 +58,9 @@ static_assert(kMergeGroup * kMergeGroup >= kAttendMaxCtas, "two levels of mergin
 template <int D, int NT>
 struct AttendCfg {
   static constexpr int kWarps = 8;
-  static constexpr int kCtas = D <= 64 || (D == 128 && NT == 1) ? 2 : 1;  // CTAs an SM: one streams while another starts or ends a unit
+  // CTAs an SM, by registers: one streams while another starts or ends a unit
+  // (128 sequences of 4000 tokens, head dim 128: 101 us, 129 with one)
+  static constexpr int kCtas = D <= 64 || (D == 128 && NT == 1) ? 2 : 1;
   static constexpr int kKSlots = 2, kVSlots = D == 512 ? 1 : 2;
   static constexpr int kVAhead = D == 512 ? 1 : 2;       // blocks that value copies run ahead
   static constexpr int kKWait = D == 512 ? 2 : 3;        // copy groups that may be pending when a block's keys are read
@@ -60,7 +71,8 @@ struct AttendCfg {
   static constexpr int kVec = D >= 128 ? 16 : 8;         // bytes of a value row a thread takes at a time
   static constexpr int kPasses = D / (8 * kVec);         // value passes of 8 threads x kVec bytes
   // What a unit's start costs, in 16-key blocks of a CTA's time: the ranges
-  // count it, so that CTAs with two units get fewer blocks.
+  // count it, so that CTAs with two units get fewer blocks (2 x 131072 tokens:
+  // 35.1 us, 41.0 without; 64 x 500: 14.7 and 17.4).
   static constexpr uint32_t kStart = D >= 256 ? 16 : 8;
 };
 
@@ -674,8 +686,9 @@ cudaError_t launch(const AttendArgs& a, uint32_t sms, int device, cudaStream_t s
 }
 
 // Two row groups a unit when sequences have more than 8 rows: the codes are
-// then converted once for 16 rows.  At head dim 512 one group's accumulators
-// already take half the registers.
+// then converted once for 16 rows (32 sequences of 4096 tokens and 32 rows,
+// head dim 128: 172 us against 198 us with one; head dim 256: 51 against 56).
+// At head dim 512 one group's accumulators already take half the registers.
 template <int D, typename T>
 cudaError_t launch_rows(const AttendArgs& a, uint32_t rows, uint32_t sms, int device, cudaStream_t s) {
   if constexpr (D < 512) {
@@ -733,11 +746,13 @@ extern "C" int q4k_paged_attention(q4k_ctx* ctx, const q4k_kv_cache* cache, cons
   a.status = ctx->select.status;
   // prompts go to the tile kernel, sequence by sequence; f32 rows keep to this one, whose f32 accuracy it lacks
   uint32_t rows = x.max_q > (1u << 24) ? 1u << 30 : (x.max_q ? x.max_q : 1) * a.group;
-  const bool prompts = x.dtype != Q4K_F32 && rows > kPromptRows;
+  const uint64_t blocks = (uint64_t)a.b.tokens * a.group / prompt_rows(a.c.dim) * a.c.heads * prompt_halves(a.c.dim);
+  const bool prompts = x.dtype != Q4K_F32 && rows > kPromptRows && blocks >= kPromptBlocks;
   a.max_rows = prompts ? kPromptRows : 0;
   const bool all = prompts && a.b.seqs == 1 && a.b.tokens * a.group > kPromptRows;  // no other sequence is left
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
+  if (all) a.max_rows = 0;  // whatever it holds is the prompt kernel's
   if (prompts) {
     e = launch_prompt(a, x.dtype, ctx->select.spin_limit, ctx->device, st);
     if (e != cudaSuccess) return ctx_cuda(ctx, e, "q4k_paged_attention prompt launch");

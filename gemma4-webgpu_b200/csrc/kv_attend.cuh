@@ -25,8 +25,21 @@ struct AttendArgs {
   uint32_t* status;
 };
 
-// Rows of a sequence and key head above which the prompt kernel takes it.
+// When the prompt kernel takes over: for sequences of more than kPromptRows rows
+// a key head, in calls whose rows fill at least kPromptBlocks of its CTAs.  It
+// cannot split a row block's keys over CTAs, so few blocks leave most SMs idle;
+// the other kernel splits, but its work grows with every 16 rows.  Measured (us,
+// prompt kernel / other), bf16:
+//   head dim 256, 2048 keys:  4 blocks 58 / 22, 16 blocks 57 / 53, 128 blocks 62 / 312
+//   head dim 256, 32768 keys: 16 blocks 729 / 538, 32 blocks 1225 / 1060, 128 blocks 1210 / 4187
+//   head dim 128, 8 heads:    16 blocks 54 / 55 and 626 / 583, 64 blocks 57 / 182 and 643 / 2293
+//   blocks of 64 of 256 rows: 84 / 56; of 128: 76 / 99
 constexpr uint32_t kPromptRows = 64;
+constexpr uint32_t kPromptBlocks = 20;
+
+// Rows of a row block, and CTAs that share one (by O's columns).
+constexpr uint32_t prompt_rows(uint32_t dim) { return dim <= 128 ? 256 : 128; }
+constexpr uint32_t prompt_halves(uint32_t dim) { return dim == 512 ? 2 : 1; }
 
 // The prompt kernel (kv_prompt.cu): sequences with more than a.max_rows rows, f16 and bf16.
 cudaError_t launch_prompt(const AttendArgs& a, uint32_t dtype, uint32_t spin, int device, cudaStream_t s);

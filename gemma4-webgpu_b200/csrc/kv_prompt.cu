@@ -29,6 +29,13 @@
 // tensor memory; at 512 a CTA computes half of O's columns and S is computed
 // by both halves (Q alone takes 128 KB of shared memory).
 //
+// Measured on B200: 4096 tokens behind 8191, 32/8 heads of 128, bf16: 824 us,
+// 835 TFLOP/s (0.51 of measured bf16); per pair of tiles the tensor cores work
+// 2500 of 4800 cycles and then wait for probabilities: a row block's own chain
+// (S, softmax, product) is longer than the other block's products.  2048 tokens
+// in a window of 512, 8/1 heads of 256: 26 us, one wave of 128 CTAs with 5 tiles
+// each; the start (rows, first codes) takes 3 us and the write 2.
+//
 // Every wait is bounded; on expiry the role records it and returns.
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -47,8 +54,8 @@ constexpr float kMostSum = 32768.0f;    // most that 64 keys' P may add up to un
 
 template <int D>
 struct PromptCfg {
-  static constexpr uint32_t kTiles = D <= 128 ? 2 : 1;
-  static constexpr uint32_t kHalves = D == 512 ? 2 : 1;           // CTAs that share a row block, by O's columns
+  static constexpr uint32_t kTiles = prompt_rows(D) / 128;
+  static constexpr uint32_t kHalves = prompt_halves(D);           // CTAs that share a row block, by O's columns
   static constexpr uint32_t kOut = D / kHalves;                    // O's columns of a CTA
   static constexpr uint32_t kChunk = D < 128 ? D : 128;            // dims of an operand chunk
   static constexpr uint32_t kKChunks = D / kChunk, kVChunks = kOut / kChunk;
@@ -200,6 +207,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) prompt_kernel(co
   const KvSeq s = kv_seq(a.b, a.c.page_shift, b);
   const uint32_t rows = s.n * G;
   const uint64_t row0_64 = ((uint64_t)slot - ((uint64_t)a.b.q_start[b] * G / RT + b)) * RT;
+  if (s.bad && tid == 0) atomicOr(a.status, kStatusKvMeta);
   if (s.bad || rows <= a.max_rows || row0_64 >= rows) return;  // served by the other kernel, or nothing
   const uint32_t row0 = (uint32_t)row0_64, n_rows = min(RT, rows - row0);
   const int pos0 = (int)s.kv - (int)s.n;

@@ -19,6 +19,13 @@
 // then inverted index, so ties go to the lowest index and no two keys are
 // equal: the result does not depend on the order of arrival.  The part that
 // finishes last merges a row's parts in their order.
+//
+// Measured on B200: 500 rows of 262144 bf16 logits, top 20: 67 us, 3.9 TB/s (0.60
+// of measured HBM; 56 us without alternatives): the exponential pass uses 0.7
+// of the issue slots.  250 f32 rows: 60 us; with a softcap 71 (two more uses of
+// the exponential unit an element).  One row: 9.5 us, the latency of the part
+// and merge steps.  Parts of up to 16 tiles (one round of CTAs) were best:
+// 73 us with two rounds, 75 with three.
 #include <cuda_runtime.h>
 #include <stdint.h>
 

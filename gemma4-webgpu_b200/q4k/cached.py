@@ -29,8 +29,8 @@ from .ops import Context, KVCache
 
 
 def rope_table(positions: int, dim: int, theta: float = 10000.0, device: torch.device | str = "cpu") -> torch.Tensor:
-    """(cos, sin) of every position and pair, f32 [positions, dim / 2, 2], from f64 angles
-    (the reference's frequencies, shaders/rope.wgsl:12)."""
+    """(cos, sin) of every position and pair, f32 [positions, dim / 2, 2], from f64
+    angles: position * theta^(-2 j / dim)."""
     freq = theta ** (-torch.arange(0, dim, 2, dtype=torch.float64, device=device) / dim)
     angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq
     return torch.stack([angle.cos(), angle.sin()], -1).float()

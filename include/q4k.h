@@ -382,8 +382,8 @@ typedef struct {
 
 /* Append the batch's new keys and values to the cache.  Keys are rotated by
  * their positions first: pairs (j, j + rope_dim/2) of the first rope_dim
- * elements of a head by rope[position][j] (the pairing of
- * shaders/rope.wgsl:14-20; store as shaders/kv_cache_store.wgsl).  With q the
+ * elements of a head by rope[position][j] (the passes of shaders/rope.wgsl
+ * and kv_cache_store.wgsl).  With q the
  * batch's queries are rotated into q_out in the same launch.  A block's scale
  * is the smallest power of two that holds its largest magnitude; it grows as
  * tokens arrive and the codes already there are rescaled, so the order and
@@ -408,7 +408,7 @@ typedef struct {
 /* Causal attention of the batch's rows over the cache: out[r][h] =
  * sum_j softmax_j(scale * q[r][h] . k[j]) v[j] over the positions j of the
  * row's sequence up to its own, the last `window` of them when window > 0
- * (shaders/attn_score.wgsl:14-39, softmax.wgsl, attn_output.wgsl:10-22).  A
+ * (shaders/attn_score.wgsl:23-30, softmax.wgsl, attn_output.wgsl).  A
  * row that sees no position is zero.  f32 rows are computed to f32 accuracy,
  * f16 and bf16 rows to that of their type, sums and softmax statistics in
  * f32 for all.  Uses the context's scratch: order the calls of one context
@@ -426,8 +426,8 @@ typedef struct {
   uint64_t stride;        /* elements from row to row */
   uint32_t dtype;
   uint32_t rows;
-  uint32_t V;
-  uint32_t top;           /* 0..32 */
+  uint32_t V;             /* at most 2^22 */
+  uint32_t top;           /* 0..32, at most V */
   float cap;              /* <= 0: none */
 } q4k_logprobs_args;
 

@@ -71,6 +71,18 @@ def test_prompts(ctx, dtype, hq, hkv, d, page, window):
     close(run(ctx, pr, dtype, window=window), pr.expected(dtype, d**-0.5, window), dtype)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hq,hkv,d,page,window", [(8, 1, 256, 32, 0), (8, 1, 512, 16, 100), (8, 2, 128, 64, 0),
+                                                  (8, 2, 128, 16, 200), (4, 4, 64, 128, 0), (5, 1, 64, 32, 50),
+                                                  (6, 2, 256, 64, 0)])
+def test_long_prompts(ctx, dtype, hq, hkv, d, page, window):
+    """Enough rows for the tile kernel at every head dim: ragged prompts behind ragged caches, with single
+    tokens, short ones and an empty sequence that are not its own."""
+    new, past = [1031, 1, 300, 0, 9, 257], [0, 75, 133, 10, 250, 1000]
+    pr = R.Problem(new, [n + p for n, p in zip(new, past)], hq, hkv, d, page, seed=5 * d + hq)
+    close(run(ctx, pr, dtype, window=window), pr.expected(dtype, d**-0.5, window), dtype)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_long_cache_is_split_and_merged(ctx, dtype):
     """One row over a cache that many CTAs share (two levels of merging), and beside short ones."""
@@ -82,17 +94,17 @@ def test_long_cache_is_split_and_merged(ctx, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("new", [1, 70, 1300])
 def test_value_blocks_of_any_magnitude(ctx, dtype, new):
-    pr = R.Problem([new], [400], 4, 1, 128, 16, seed=21, v_mix=True)
+    pr = R.Problem([new], [max(400, new + 31)], 4, 1, 128, 16, seed=21, v_mix=True)
     close(run(ctx, pr, dtype), pr.expected(dtype, 128**-0.5), dtype)
 
 
 @pytest.mark.parametrize("dtype", [F32, F16])
-@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("new", [1, 40, 1400])
 def test_peaked_flat_and_scaled_rows(ctx, dtype, new):
     """Rows of zeros (flat weights), of large scores (one key decides) and of tiny and large magnitude."""
-    pr = R.Problem([new], [300], 4, 1, 64, 32, seed=23, spread=1.0)
+    pr = R.Problem([new], [max(300, new)], 4, 1, 64, 32, seed=23, spread=1.0)
     pr.q[:, 0] = 0.0
     pr.q[:, 1] *= 8.0
     pr.q[:, 2] *= 1e-3
@@ -103,7 +115,7 @@ def test_peaked_flat_and_scaled_rows(ctx, dtype, new):
     assert float((got[:, 1] - want[:, 1]).norm()) <= 8 * NORM[dtype] * float(want[:, 1].norm())
 
 
-@pytest.mark.parametrize("new", [1, 64])
+@pytest.mark.parametrize("new", [1, 64, 700])
 def test_what_is_masked_does_not_matter(ctx, new):
     """Slots past the end may hold anything, NaN codes and scales among it;
     rows of other sequences may be NaN."""
@@ -126,17 +138,17 @@ def test_what_is_masked_does_not_matter(ctx, new):
     assert torch.isnan(got[new:]).all()
 
 
-@pytest.mark.parametrize("new", [1, 30])
-def test_no_position_no_weight(ctx, new):
+@pytest.mark.parametrize("new,dtype", [(1, F32), (30, F32), (1400, BF16)])
+def test_no_position_no_weight(ctx, new, dtype):
     """More new rows than tokens in the cache: the first rows have no position and are zero."""
     pr = R.Problem([new], [max(0, new - 5)], 4, 1, 64, 16, seed=37)
-    got = run(ctx, pr, F32).cpu()
+    got = run(ctx, pr, dtype).cpu()
     none = min(5, new)
     assert (got[:none] == 0).all()
     if new > 5:
         sub = R.Problem([new - 5], [new - 5], 4, 1, 64, 16, seed=37)
         sub.q, sub.k, sub.v, sub.k_scale, sub.v_scale, sub.table = pr.q[5:], pr.k, pr.v, pr.k_scale, pr.v_scale, pr.table
-        close(got[5:], sub.expected(F32, 64**-0.5), F32)
+        close(got[5:], sub.expected(dtype, 64**-0.5), dtype)
 
 
 def test_strides_streams_and_shared_pages(ctx):
@@ -160,16 +172,16 @@ def test_strides_streams_and_shared_pages(ctx):
 
 
 def test_max_q_is_a_hint(ctx):
-    pr = R.Problem([50, 1], [80, 30], 8, 1, 128, 32, seed=43)
+    pr = R.Problem([700, 1, 80], [730, 30, 80], 8, 1, 128, 32, seed=43)
     import q4k
 
     want = pr.expected(F16, 128**-0.5)
     cache, q, table, qs, kvl = pr.device(DEV, q4k, F16)
-    for hint in (0, 1, 49, 500):
+    for hint in (0, 1, 70, 699, 700, 5000):
         close(ctx.paged_attention(cache, q, table, qs, kvl, hint, 128**-0.5), want, F16)
 
 
-@pytest.mark.parametrize("new", [1, 64])
+@pytest.mark.parametrize("new", [1, 64, 400])
 @pytest.mark.parametrize("what", ["page", "length", "rows"])
 def test_bad_metadata_is_reported(ctx, what, new):
     import q4k
@@ -190,6 +202,28 @@ def test_bad_metadata_is_reported(ctx, what, new):
         close(got[:new], want[:new], BF16)
     else:
         close(got[new:], want[new:], BF16)
+
+
+@pytest.mark.parametrize("new", [1, 700])
+def test_bad_metadata_of_the_only_sequence(ctx, new):
+    import q4k
+
+    pr = R.Problem([new], [new + 9], 8, 1, 128, 16, seed=53)
+    cache, q, table, qs, kvl = pr.device(DEV, q4k, BF16)
+    kvl[0] = 1 << 20
+    ctx.paged_attention(cache, q, table, qs, kvl, new, 128**-0.5)
+    with pytest.raises(q4k.Q4KError, match="out of range"):
+        ctx.check()
+    kvl[0] = new + 9
+    qs[1] = max(1, new // 350)  # fewer rows than the buffer holds: the others are left alone
+    out = torch.full_like(q, 3.0)
+    ctx.paged_attention(cache, q, table, qs, kvl, new, 128**-0.5, out=out)
+    ctx.check()
+    n = int(qs[1])
+    sub = R.Problem([n], [new + 9], 8, 1, 128, 16, seed=53)
+    sub.q, sub.k, sub.v, sub.k_scale, sub.v_scale, sub.table = pr.q[:n], pr.k, pr.v, pr.k_scale, pr.v_scale, pr.table
+    close(out[:n], sub.expected(BF16, 128**-0.5), BF16)
+    assert (out[n:] == 3).all()
 
 
 def test_refusals(ctx):
