@@ -19,7 +19,7 @@
 // Measured on B200: 16384 tokens of 32 query and 8 key heads of 128 (bf16)
 // 86 us, 4.4 TB/s; of these the queries take 40 us, the speed of a plain copy,
 // the keys and values 46 us, bound by a CTA's chain of loads (metadata, rows
-// and page, scale) at 7 CTAs an SM.  5 ragged prompts 8.9 us, 64 single tokens
+// and page, scale) at 9 CTAs an SM.  5 ragged prompts 8.9 us, 64 single tokens
 // 5.3 us, one 3.0 us (latency of the same chain).
 #include <cuda_runtime.h>
 #include <stdint.h>
