@@ -725,6 +725,7 @@ extern "C" int q4k_paged_attention(q4k_ctx* ctx, const q4k_kv_cache* cache, cons
     return Q4K_OK;
   }
   if (!x.q || !x.out) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: null pointer");
+  if (x.q == x.out) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: out must not overlap q");
   if (x.q_heads == 0) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: q_heads must be >= 1");
   if (!(x.scale == x.scale) || fabsf(x.scale) > 3.402823466e38f)
     return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_paged_attention: scale must be finite");

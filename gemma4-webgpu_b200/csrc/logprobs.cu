@@ -22,8 +22,8 @@
 //
 // Measured on B200: 500 rows of 262144 bf16 logits, top 20: 67 us, 3.9 TB/s (0.60
 // of measured HBM; 56 us without alternatives): the exponential pass uses 0.7
-// of the issue slots.  250 f32 rows: 60 us; with a softcap 71 (two more uses of
-// the exponential unit an element).  One row: 9.5 us, the latency of the part
+// of the issue slots; 94 us with a softcap, 117 without its polynomial.  250 f32
+// rows: 60 us, 64 with a softcap.  One row: 9.5 us, the latency of the part
 // and merge steps.  Parts of up to 16 tiles (one round of CTAs) were best:
 // 73 us with two rounds, 75 with three.
 #include <cuda_runtime.h>
@@ -56,7 +56,7 @@ struct LpArgs {
   uint64_t stride;
   uint32_t row0, V, splits, top;  // row0: first row of this launch
   uint32_t part_vecs;             // 16-byte vectors of a part, a multiple of kLpThreads
-  float cap, cap_rate;  // 0: none; 2 log2(e) / cap
+  float cap, cap_rate, cap_inv;  // 0: none; 2 log2(e) / cap; 1 / cap
   const int32_t* tokens;
   float* logprob;
   float* entropy;
@@ -93,11 +93,20 @@ __device__ __forceinline__ unsigned long long key_of(float x, uint32_t idx) {
   return ((unsigned long long)ord_of(x) << 32) | (0xffffffffu - idx);
 }
 
-// A logit's softcapped value: cap tanh(v / cap) = cap - 2 cap / (2^(2 log2(e) v / cap) + 1).
+// tanh(y) / y on |y| <= 1/2 as a polynomial in y^2 (least relative error,
+// 1.3e-8, by weighted least squares on Chebyshev points).
+constexpr float kT0 = 1.0f, kT1 = -0.3333307f, kT2 = 0.1332478f, kT3 = -0.05298607f, kT4 = 0.017135f;
+
+// A logit's softcapped value cap tanh(v / cap).  Small |v| / cap, where most
+// logits are, by the polynomial: no use of the exponential unit, and exact for
+// a cap far above the logits; else cap - 2 cap / (2^(2 log2(e) v / cap) + 1).
 template <bool kCap>
 __device__ __forceinline__ float capped(float v, const LpArgs& a) {
   if (!kCap) return v;
-  return fmaf(-2.0f * a.cap, __fdividef(1.0f, lp_ex2(v * a.cap_rate) + 1.0f), a.cap);
+  const float y = v * a.cap_inv, y2 = y * y;
+  const float small = v * fmaf(fmaf(fmaf(fmaf(kT4, y2, kT3), y2, kT2), y2, kT1), y2, kT0);
+  const float large = fmaf(-2.0f * a.cap, __fdividef(1.0f, lp_ex2(v * a.cap_rate) + 1.0f), a.cap);
+  return fabsf(y) <= 0.5f ? small : large;
 }
 
 // The elements of a 16-byte vector.
@@ -134,6 +143,14 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 r;
   asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return r;
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
       : "=l"(reinterpret_cast<unsigned long long&>(r))
       : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
   return r;
@@ -242,14 +259,17 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a)
       const uint32_t v = v0 + (kLpVecs + i) * kLpThreads;
       if (v < v_hi) raw[i] = ldg_nc_v4(xv + (uint64_t)v * kVE);
     }
-    float mx = __int_as_float(0x7fc00000);
+    float mx = __int_as_float(0x7fc00000), mn = mx;  // (fmaxf and fminf pass over NaN)
 #pragma unroll
     for (uint32_t i = 0; i < kLpVecs; ++i) {
       if (v0 + i * kLpThreads < v_hi) {
         float e[kVE];
         unpack(cur[i], e, kTag);
 #pragma unroll
-        for (uint32_t j = 0; j < kVE; ++j) mx = fmaxf(mx, e[j]);
+        for (uint32_t j = 0; j < kVE; ++j) {
+          mx = fmaxf(mx, e[j]);
+          if (kCap) mn = fminf(mn, e[j]);
+        }
       }
     }
     any = true;
@@ -260,19 +280,34 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a)
     const float ref = -st.m * kLog2e;
     float2 ss = make_float2(0.0f, 0.0f), ws = ss;
     const float2 ref2 = make_float2(ref, ref), rate2 = make_float2(kLog2e, kLog2e);
+    auto add_tile = [&](auto value2) {
 #pragma unroll
-    for (uint32_t i = 0; i < kLpVecs; ++i) {
-      if (v0 + i * kLpThreads < v_hi) {
-        float e[kVE];
-        unpack(cur[i], e, kTag);
+      for (uint32_t i = 0; i < kLpVecs; ++i) {
+        if (v0 + i * kLpThreads < v_hi) {
+          float e[kVE];
+          unpack(cur[i], e, kTag);
 #pragma unroll
-        for (uint32_t j = 0; j < kVE; j += 2) {
-          const float2 d = fma2(make_float2(capped<kCap>(e[j], a), capped<kCap>(e[j + 1], a)), rate2, ref2);
-          const float2 p = make_float2(lp_ex2(d.x), lp_ex2(d.y));
-          ss = add2(ss, p);
-          ws = fma2(p, d, ws);
+          for (uint32_t j = 0; j < kVE; j += 2) {
+            const float2 d = fma2(value2(make_float2(e[j], e[j + 1])), rate2, ref2);
+            const float2 p = make_float2(lp_ex2(d.x), lp_ex2(d.y));
+            ss = add2(ss, p);
+            ws = fma2(p, d, ws);
+          }
         }
       }
+    };
+    if constexpr (!kCap) {
+      add_tile([](float2 v) { return v; });
+    } else if (mx <= 0.5f * a.cap && mn >= -0.5f * a.cap) {
+      add_tile([&](float2 v) {
+        const float2 y = mul2(v, make_float2(a.cap_inv, a.cap_inv)), y2 = mul2(y, y);
+        float2 t = fma2(make_float2(kT4, kT4), y2, make_float2(kT3, kT3));
+        t = fma2(t, y2, make_float2(kT2, kT2));
+        t = fma2(t, y2, make_float2(kT1, kT1));
+        return mul2(v, fma2(t, y2, make_float2(kT0, kT0)));
+      });
+    } else {
+      add_tile([&](float2 v) { return make_float2(capped<true>(v.x, a), capped<true>(v.y, a)); });
     }
     float s0 = ss.x + ss.y, w0 = ws.x + ws.y;
     if (!(fabsf(w0) <= 3.402823466e38f)) {  // -inf, NaN, or values near the end of f32's range: term by term
@@ -539,7 +574,8 @@ extern "C" int q4k_token_logprobs(q4k_ctx* ctx, const q4k_logprobs_args* args, v
   if (x.top > kLpTop || x.top > x.V)
     return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: top=%u above %u or V=%u", x.top, kLpTop, x.V);
   if (x.stride < x.V) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: stride below V=%u", x.V);
-  if (!(x.cap == x.cap)) return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: cap is NaN");
+  if (!(fabsf(x.cap) <= 3.402823466e38f) || (x.cap > 0.0f && x.cap < 1e-30f))
+    return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: cap must be finite, and not below 1e-30 when positive");
   if ((uintptr_t)x.logits % dtype_bytes(x.dtype))
     return ctx_fail(ctx, Q4K_ERR_INVALID_ARG, "q4k_token_logprobs: logits not aligned to their type");
   LpArgs a{};
@@ -557,6 +593,7 @@ extern "C" int q4k_token_logprobs(q4k_ctx* ctx, const q4k_logprobs_args* args, v
   a.counters = ctx->split_counters;
   a.status = ctx->select.status;
   a.cap_rate = a.cap > 0.0f ? 2.0f * kLog2e / a.cap : 0.0f;
+  a.cap_inv = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const uint32_t sms = (uint32_t)ctx->sm_count;
   cudaError_t e;

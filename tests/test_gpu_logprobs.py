@@ -150,6 +150,15 @@ def test_large_magnitudes(ctx):
     check(ctx, x * 1e4, torch.tensor([1, 2], dtype=torch.int32), 3, cap=30.0)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cap", [0.5, 5.0, 50.0, 1e4])
+def test_caps_of_any_size(ctx, dtype, cap):
+    """Caps that most logits exceed, that some do, and that none comes near; masked logits become -cap."""
+    x = (torch.randn(3, 30000, generator=torch.Generator().manual_seed(2)) * 6).to(dtype)
+    x[1, ::3] = -math.inf
+    check(ctx, x, torch.tensor([5, 6, 7], dtype=torch.int32), 10, cap)
+
+
 def test_refusals(ctx):
     import q4k
 
@@ -161,7 +170,8 @@ def test_refusals(ctx):
     for top in (-1, 33, 101):
         with pytest.raises(ValueError):
             ctx.token_logprobs(x, t, top=top)
-    with pytest.raises(q4k.Q4KError):
-        ctx.token_logprobs(x, t, cap=float("nan"))
+    for cap in (float("nan"), float("inf"), 1e-38):
+        with pytest.raises(q4k.Q4KError):
+            ctx.token_logprobs(x, t, cap=cap)
     assert ctx.token_logprobs(x[:0], t[:0], top=3)[3].shape == (0, 3)
     ctx.check()

@@ -237,7 +237,7 @@ def test_refusals(ctx):
         (dict(q=q[:, :, :32]), ValueError), (dict(out=torch.empty_like(q).half()), TypeError),
         (dict(window=-1), ValueError), (dict(max_q=-1), ValueError), (dict(scale=float("nan")), q4k.Q4KError),
         (dict(kv_len=kvl.long()), TypeError), (dict(block_table=table.cpu()), ValueError),
-        (dict(q_start=qs[:1]), ValueError), (dict(q=q.cpu()), ValueError),
+        (dict(q_start=qs[:1]), ValueError), (dict(q=q.cpu()), ValueError), (dict(out=q), q4k.Q4KError),
     ]:
         with pytest.raises(err):
             ctx.paged_attention(**{**ok, **change})
