@@ -11,16 +11,20 @@
 //     theirs: E never falls while the block fills), code = e4m3(x' / 2^E),
 //     nearest even; a block whose scale changes has its other slots recoded.
 //
-// One CTA owns one block of one sequence and head: its new rows stay in
-// registers (16 values a thread) between the maximum and the codes, so k, v
-// are read once and the codes written once, and nothing is shared between
-// CTAs.  Only when the scale changes are the block's other codes read back.
+// One CTA owns one block of one sequence for up to 4 heads, one after the other:
+// a head's new rows stay in registers (16 values a thread) between the maximum
+// and the codes, the next head's rows on their way, so k, v are read once and
+// the codes written once, and nothing is shared between CTAs.  Only when the
+// scale changes are the block's other codes read back.
 //
 // Measured on B200: 16384 tokens of 32 query and 8 key heads of 128 (bf16)
-// 86 us, 4.4 TB/s; of these the queries take 40 us, the speed of a plain copy,
-// the keys and values 46 us, bound by a CTA's chain of loads (metadata, rows
-// and page, scale) at 9 CTAs an SM.  5 ragged prompts 8.9 us, 64 single tokens
-// 5.3 us, one 3.0 us (latency of the same chain).
+// 76 us, 5.0 TB/s (0.77 of measured HBM): the queries alone run at the speed of
+// a plain copy, the keys and values alone take 31 us (46 with one head a CTA,
+// whose chain of loads, metadata, page and rows, then shows; 73 us in all with
+// 8 heads, but a single token's heads would wait for one another).  5 ragged
+// prompts 8.9 us, 64 single tokens 5.5 us, one 3.0 us (latency of that chain).
+// Registers are held to 64: at 90 and more the queries lose their occupancy
+// (93 us).
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -29,7 +33,8 @@
 namespace q4k {
 namespace {
 
-constexpr uint32_t kQHeadsPerCta = 4;  // query heads that share a thread's (cos, sin)
+constexpr uint32_t kQHeadsPerCta = 4;   // query heads that share a thread's (cos, sin)
+constexpr uint32_t kKvHeadsPerCta = 4;  // key (or value) heads of a CTA, one after the other
 
 struct AppendArgs {
   KvCache c;
@@ -99,10 +104,10 @@ __device__ __forceinline__ float finite(float x, bool* bad) {
 
 // grid.x: block slots (sequence b's start at q_start[b] / 16 + 2 b, which
 // leaves each sequence room for every block that its n tokens can touch, so
-// no prefix sum is needed); grid.y: key heads, value heads, groups of query
-// heads.  blockDim.x = head dim: one item (16 values) of one token a thread.
+// no prefix sum is needed); grid.y: groups of key heads, of value heads,
+// of query heads.  blockDim.x = head dim: one item (16 values) of one token a thread.
 template <typename T>
-__global__ void __launch_bounds__(512) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(512, 2) append_kernel(const AppendArgs a) {
   const uint32_t D = a.c.dim, H = a.c.heads, per = D / 16;
   // the block's sequence: the last one that starts at or before this slot.  Its
   // thread has loaded the values along, so one round of loads tells all.
@@ -146,7 +151,8 @@ __global__ void __launch_bounds__(512) append_kernel(const AppendArgs a) {
   const uint64_t row = s.t0 + skip + (pos - p0);
   uint32_t role = blockIdx.y;
   uint32_t lo, hi;
-  if (role >= 2 * H) {  // queries
+  const uint32_t groups = (H + kKvHeadsPerCta - 1) / kKvHeadsPerCta;
+  if (role >= 2 * groups) {  // queries
     if (!mine) return;
     item_at(item, a.rot, &lo, &hi);
     const bool turn = 8 * item < a.rot / 2;
@@ -156,7 +162,7 @@ __global__ void __launch_bounds__(512) append_kernel(const AppendArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) cs[j] = __ldg(t + j);
     }
-    const uint32_t h0 = (role - 2 * H) * kQHeadsPerCta;
+    const uint32_t h0 = (role - 2 * groups) * kQHeadsPerCta;
     const T* src = static_cast<const T*>(a.q) + row * a.q_stride;
     T* dst = static_cast<T*>(a.q_out) + row * a.qo_stride;
 #pragma unroll
@@ -171,24 +177,57 @@ __global__ void __launch_bounds__(512) append_kernel(const AppendArgs a) {
     }
     return;
   }
-  const bool is_v = role >= H;
-  const uint32_t h = is_v ? role - H : role;
+  const bool is_v = role >= groups;
+  const uint32_t h0 = (is_v ? role - groups : role) * kKvHeadsPerCta, n_heads = min(kKvHeadsPerCta, H - h0);
   const uint32_t rot = is_v ? 0 : a.rot;
   item_at(item, rot, &lo, &hi);
-  float x[8] = {}, y[8] = {};
-  bool bad = false;
-  float mx = 0.0f;
-  if (mine) {
-    const T* src = static_cast<const T*>(is_v ? a.v : a.k) + row * (is_v ? a.v_stride : a.k_stride) + h * D;
-    load_elems(src + lo, x);
-    load_elems(src + hi, y);
-    if (8 * item < rot / 2) {
-      const float4* t = reinterpret_cast<const float4*>(a.rope + ((uint64_t)pos * (rot / 2) + 8 * item) * 2);
-      float4 cs[4];
+  const uint32_t page = a.b.table[(uint64_t)b * a.b.cols + (bs >> a.c.page_shift)];
+  uint64_t blk0;
+  const bool ok = kv_block(a.c, page, h0, bs, &blk0);
+  if (!ok) {
+    if (threadIdx.x == 0) atomicOr(a.status, kStatusKvMeta);
+    return;
+  }
+  const uint32_t per_head = 1u << (a.c.page_shift - 4);  // blocks from one head to the next
+  float* const scales = (is_v ? a.c.vs : a.c.ks) + blk0;
+  const bool fresh = p0 <= bs;  // the block's first token comes now
+  const bool whole = fresh && bs + 16 <= s.kv && !(a.rot && bs + 16 > a.rope_len);  // and all the others
+  float4 cs[4];
+  const bool turn = mine && 8 * item < rot / 2;
+  if (turn) {
+    const float4* t = reinterpret_cast<const float4*>(a.rope + ((uint64_t)pos * (rot / 2) + 8 * item) * 2);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) cs[j] = __ldg(t + j);
-      rotate8(x, y, cs);
+    for (int j = 0; j < 4; ++j) cs[j] = __ldg(t + j);
+  }
+  // head by head, the next one's rows (and the scale in place, which a block
+  // that is new as a whole does not need) on their way
+  constexpr int kWords = 8 * sizeof(T) / 16;
+  __shared__ uint32_t s_max[2][16];
+  uint4 raw[2 * kWords] = {}, next[2 * kWords] = {};
+  float old = 0.0f, old_next = 0.0f;
+  const T* const src = static_cast<const T*>(is_v ? a.v : a.k) + row * (is_v ? a.v_stride : a.k_stride) + h0 * D;
+  auto fetch = [&](uint32_t k) {
+    if (mine) {
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        next[w] = reinterpret_cast<const uint4*>(src + k * D + lo)[w];
+        next[kWords + w] = reinterpret_cast<const uint4*>(src + k * D + hi)[w];
+      }
     }
+    if (!whole) old_next = scales[k * per_head];
+  };
+  fetch(0);
+  bool bad = false;
+#pragma unroll 1
+  for (uint32_t k = 0; k < n_heads; ++k) {
+#pragma unroll
+    for (int w = 0; w < 2 * kWords; ++w) raw[w] = next[w];
+    old = old_next;
+    if (k + 1 < n_heads) fetch(k + 1);
+    float x[8], y[8], mx = 0.0f;
+    load_elems(reinterpret_cast<const T*>(&raw[0]), x);
+    load_elems(reinterpret_cast<const T*>(&raw[kWords]), y);
+    if (turn) rotate8(x, y, cs);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       x[j] = finite(x[j], &bad);
@@ -197,44 +236,33 @@ __global__ void __launch_bounds__(512) append_kernel(const AppendArgs a) {
       if (fabsf(x[j]) < 3.4e38f) mx = fmaxf(mx, fabsf(x[j]));
       if (fabsf(y[j]) < 3.4e38f) mx = fmaxf(mx, fabsf(y[j]));
     }
+    // the block's largest magnitude (as bits: they order like the values)
+    const uint32_t wm = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
+    if ((threadIdx.x & 31) == 0) s_max[k & 1u][threadIdx.x >> 5] = wm;
+    __syncthreads();
+    uint32_t m = s_max[k & 1u][0];
+    for (uint32_t i = 1; i < blockDim.x / 32; ++i) m = max(m, s_max[k & 1u][i]);
+    int e = kv_scale_exp(__uint_as_float(m));
+    const int e_old = exp_of(old);
+    if (!fresh) e = max(e, e_old);
+    uint8_t* const base = (is_v ? a.c.v : a.c.k) + (blk0 + k * per_head) * (16 * D) + (uint64_t)(pos - bs) * D;
+    if (mine) {
+      const float inv = exp2i(-e);
+      *reinterpret_cast<uint2*>(base + lo) = codes8(x, inv);
+      *reinterpret_cast<uint2*>(base + hi) = codes8(y, inv);
+    } else if (e != e_old) {  // (not in a whole block: every slot has a new token)
+      // a slot without a new token: an older token's, or one past the end whose
+      // stale content a fresh block's smaller scale may not hold (then NaN; no
+      // position has it yet)
+      const float ratio = exp2i(min(max(e_old - e, -126), 127));
+      uint2* u = reinterpret_cast<uint2*>(base + lo);
+      uint2* w = reinterpret_cast<uint2*>(base + hi);
+      *u = make_uint2(recode4(u->x, ratio), recode4(u->y, ratio));
+      *w = make_uint2(recode4(w->x, ratio), recode4(w->y, ratio));
+    }
+    if (threadIdx.x == 0 && (whole || e != e_old)) scales[k * per_head] = exp2i(e);
   }
   if (bad) atomicOr(a.status, kStatusKvNonFinite);
-  // the block's largest magnitude (as bits: they order like the values)
-  __shared__ uint32_t s_max[16];
-  const uint32_t wm = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = wm;
-  const uint32_t page = a.b.table[(uint64_t)b * a.b.cols + (bs >> a.c.page_shift)];
-  uint64_t blk;
-  const bool ok = kv_block(a.c, page, h, bs, &blk);
-  float* const sp = (is_v ? a.c.vs : a.c.ks) + blk;
-  const bool fresh = p0 <= bs;  // the block's first token comes now
-  const float old = ok ? *sp : 0.0f;
-  __syncthreads();
-  if (!ok) {
-    if (threadIdx.x == 0) atomicOr(a.status, kStatusKvMeta);
-    return;
-  }
-  uint32_t m = s_max[0];
-  for (uint32_t i = 1; i < blockDim.x / 32; ++i) m = max(m, s_max[i]);
-  int e = kv_scale_exp(__uint_as_float(m));
-  const int e_old = exp_of(old);
-  if (!fresh) e = max(e, e_old);
-  uint8_t* const base = (is_v ? a.c.v : a.c.k) + blk * (16 * D) + (uint64_t)(pos - bs) * D;
-  if (mine) {
-    const float inv = exp2i(-e);
-    *reinterpret_cast<uint2*>(base + lo) = codes8(x, inv);
-    *reinterpret_cast<uint2*>(base + hi) = codes8(y, inv);
-  } else if (e != e_old) {
-    // a slot without a new token: an older token's, or one past the end whose
-    // stale content a fresh block's smaller scale may not hold (then NaN; no
-    // position has it yet)
-    const float ratio = exp2i(min(max(e_old - e, -126), 127));
-    uint2* u = reinterpret_cast<uint2*>(base + lo);
-    uint2* w = reinterpret_cast<uint2*>(base + hi);
-    *u = make_uint2(recode4(u->x, ratio), recode4(u->y, ratio));
-    *w = make_uint2(recode4(w->x, ratio), recode4(w->y, ratio));
-  }
-  if (threadIdx.x == 0 && e != e_old) *sp = exp2i(e);
 }
 
 }  // namespace
@@ -324,7 +352,9 @@ extern "C" int q4k_kv_append(q4k_ctx* ctx, const q4k_kv_cache* cache, const q4k_
   a.rope_len = x.rope_len;
   a.rot = x.rope_dim;
   a.status = ctx->select.status;
-  const dim3 grid(a.b.tokens / 16 + 2 * a.b.seqs + 1, 2 * a.c.heads + (a.q_heads + kQHeadsPerCta - 1) / kQHeadsPerCta);
+  const dim3 grid(a.b.tokens / 16 + 2 * a.b.seqs + 1,
+                  2 * ((a.c.heads + kKvHeadsPerCta - 1) / kKvHeadsPerCta) +
+                      (a.q_heads + kQHeadsPerCta - 1) / kQHeadsPerCta);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (x.dtype == Q4K_F32)
     append_kernel<float><<<grid, D, 0, st>>>(a);
