@@ -102,6 +102,21 @@ def test_codes_scales_and_queries(ctx, dtype, new, past, hq, hkv, d, page, rot):
                 3 * 2.0**-23) * q[t].double().abs().amax()).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("hkv,d", [(4, 128), (5, 64), (8, 256), (9, 128), (6, 512)])
+def test_many_heads(ctx, dtype, hkv, d):
+    """Heads that share a CTA, whole groups and a last one that is not full, each
+    head's rows 2^h larger than the last: a scale of its own in every block."""
+    new, past = [40, 1, 3], [9, 31, 0]
+    q4k, pr, k, v, _, rope = make(new, past, hkv, hkv, d, 32, 64, dtype, seed=hkv)
+    grow = (2.0 ** torch.arange(hkv)).to(dtype)[:, None]
+    k, v = k * grow, v * grow
+    cache, _, table, qs, kvl = pr.device(DEV, q4k, dtype)
+    ctx.kv_append(cache, k.to(DEV), v.to(DEV), rope.to(DEV), table, qs, kvl)
+    ctx.check()
+    check(pr, cache, k, v, rope, past)
+
+
 def test_one_by_one_equals_at_once(ctx):
     """Power-of-two scales: growth only shifts exponents, so the caches agree
     wherever a code is not subnormal (below 2^-6 of the scale)."""
